@@ -123,6 +123,11 @@ SIGNATURES = {
     'glmvx_argmax_rows': ([_P, _P, _I32, _I32, _P], _I32),
     'glmvx_fill_random': ([_P, _I32, _I64, _U64, _F32, _I32, _P], _I32),
     'glmvx_dsa_attend': ([_P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _F32, _P, _U64, _P], _I32),
+    'glmvx_lora_workspace_bytes': ([_I32, _I32, _I32], _I64),
+    'glmvx_lora_add': ([_P, _I64, _P, _I64, _P, _I32, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _P, _U64, _P],
+                       _I32),
+    'glmvx_logits_select': ([_P, _P, _I64, _P, _I64, _I32, _I32, _P, _P, _I32, _P, _P, _P, _P, _P, _P, _I32, _P, _P,
+                             _I32, _P], _I32),
     'glmvx_moe_job_counts': ([_I32, _I32, _I32, _I32, _I32, _I32, _P, _PI32, _P], _I32),
 }
 

@@ -381,6 +381,56 @@ int32_t glmvx_dsa_attend(float *out, const int32_t *selected, const float *q_lat
                          const float *latents, const float *rope_keys, const int32_t *lens, int32_t batch,
                          int32_t heads, int32_t rank, int32_t rope_dim, int32_t capacity, int32_t topk, float scale,
                          void *scratch, uint64_t scratch_bytes, void *stream);
+/* Low-rank adapters of many requests beside a shared projection, for a batch
+ * whose rows belong to different requests (the reference serves one set of
+ * weights; no counterpart):
+ *   y[t] += scales[a] * B_a (A_a x[t]),  a = adapter_ids[t], t < tokens
+ * x[t][cols] and y[t][rows] f32 with row strides in elements (columns
+ * contiguous); adapter_ids -1 (any negative): the row stays as it is, and an
+ * id >= adapters leaves it too and sets the device error word (3).
+ * a: [adapters][max_rank][cols], b: [adapters][rows][max_rank], both of one
+ * GGML kind: 0 F32, 1 F16, 30 BF16; of adapter a the first ranks[a] (0 ..
+ * max_rank, clamped) rows of A and columns of B are read, the rest may hold
+ * anything.  Products and sums are f32 whatever the kind.  A token's result
+ * does not depend on the other tokens' adapters and is the same every time.
+ * tokens <= 2^20, max_rank <= 256.  y must not overlap x.  workspace: device
+ * scratch of glmvx_lora_workspace_bytes(...) bytes, 16-byte aligned; calls
+ * that may overlap in time need one each. */
+int64_t glmvx_lora_workspace_bytes(int32_t tokens, int32_t adapters, int32_t max_rank);
+int32_t glmvx_lora_add(float *y, int64_t y_stride, const float *x, int64_t x_stride, const int32_t *adapter_ids,
+                       int32_t kind, const void *a, const void *b, const int32_t *ranks, const float *scales,
+                       int32_t tokens, int32_t rows, int32_t cols, int32_t adapters, int32_t max_rank,
+                       void *workspace, uint64_t workspace_bytes, void *stream);
+/* Each row's next token under its request's rules (the reference samples from
+ * the model's logits as they are, glm_vx/scheduler.py:113-120; no
+ * counterpart).  Row b's logits l[v], in f32 with one rounding per operation:
+ *   v in the history, or fed:       l = l > 0 ? l / repetition : l * repetition
+ *   v c > 0 times among the output: l = l - c * frequency - presence
+ *   v biased:                       l = l + bias
+ *   mask bit of v clear:            l = -inf
+ * go to out[b][v] (out may be logits), and the lowest index of the largest to
+ * selected[b] (the first NaN when there is one, as numpy's argmax; -1 when
+ * nothing is above -inf).  Strides in elements.  Each group may be NULL:
+ *   history   history[b][history_capacity] token ids, the first
+ *             history_lens[b] valid, of those the first prompt_lens[b] (NULL:
+ *             none) the prompt, the rest output; ids outside the vocabulary
+ *             are skipped.  fed[b] (NULL: none; negative: none for this row)
+ *             is the token the row was just fed: it counts as the history's
+ *             next entry and, while there is room, is appended to it.
+ *   penalties [rows][3] repetition (> 0; 1 none), presence, frequency (0 none)
+ *   biases    row b's first bias_lens[b] of bias_ids / bias_values
+ *             [rows][bias_capacity]; of a token's entries the last one holds
+ *   masks     [mask_count][ceil(vocab/32)] words, bit v % 32 of word v / 32
+ *             set: v is allowed; row b uses mask mask_rows[b], none if that
+ *             is negative; beyond mask_count nothing is allowed and the
+ *             device error word is set (3), as it is by a fed token >= vocab.
+ * history_capacity <= 2^20 - 2, bias_capacity <= 2047.  selected may be fed. */
+int32_t glmvx_logits_select(int32_t *selected, float *out, int64_t out_stride, const float *logits,
+                            int64_t logits_stride, int32_t rows, int32_t vocab, const int32_t *fed, int32_t *history,
+                            int32_t history_capacity, int32_t *history_lens, const int32_t *prompt_lens,
+                            const float *penalties, const int32_t *bias_ids, const float *bias_values,
+                            const int32_t *bias_lens, int32_t bias_capacity, const uint32_t *masks,
+                            const int32_t *mask_rows, int32_t mask_count, void *stream);
 /* FP8 E4M3FN block-scaled projection, device pointers: out[rows] =
  * sum_c (decode(weight[r,c]) * scales[r/128, c/128]) * x[c], weight u8
  * [rows, cols], scales f32 [ceil(rows/128), ceil(cols/128)].  Replaces the
