@@ -424,7 +424,8 @@ int32_t glmvx_lora_add(float *y, int64_t y_stride, const float *x, int64_t x_str
  *             set: v is allowed; row b uses mask mask_rows[b], none if that
  *             is negative; beyond mask_count nothing is allowed and the
  *             device error word is set (3), as it is by a fed token >= vocab.
- * history_capacity <= 2^20 - 2, bias_capacity <= 2047.  selected may be fed. */
+ * vocab <= 2^30, rows <= 2^24, history_capacity <= 2^20 - 2, bias_capacity <=
+ * 2047.  selected may be fed. */
 int32_t glmvx_logits_select(int32_t *selected, float *out, int64_t out_stride, const float *logits,
                             int64_t logits_stride, int32_t rows, int32_t vocab, const int32_t *fed, int32_t *history,
                             int32_t history_capacity, int32_t *history_lens, const int32_t *prompt_lens,

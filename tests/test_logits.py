@@ -15,7 +15,8 @@ def call(**change):
 
 
 @pytest.mark.parametrize('change,message', [
-    (dict(rows=-1), 'dimensions'), (dict(vocab=0), 'dimensions'), (dict(selected=None), 'null'),
+    (dict(rows=-1), 'dimensions'), (dict(vocab=0), 'dimensions'), (dict(vocab=2**30 + 1), 'dimensions'),
+    (dict(rows=2**24 + 1), 'dimensions'), (dict(selected=None), 'null'),
     (dict(out=None), 'null'), (dict(logits=None), 'null'), (dict(out_stride=99), 'strides'),
     (dict(logits_stride=99), 'strides'), (dict(out=8192, out_stride=101), 'in place'),
     (dict(history=None), 'history'), (dict(history_lens=None), 'history'),
