@@ -1,13 +1,27 @@
 // Low-rank adapters of many requests beside a shared projection:
 //   y[t] += s_a * B_a (A_a x[t]),   a = adapter_ids[t]  (-1: none, row t stays)
 // with A_a [rank_a][cols] and B_a [rows][rank_a] taken from stacks padded to
-// max_rank.  Two kernels: lora_shrink (h = A x, f32, into the workspace) and
-// lora_expand (y += s B h).  Sums are f32; weights are F32, F16 or BF16 and
-// widen to f32 exactly.
+// max_rank.  Two kernels: lora_shrink (h = A x, f32, into the workspace, the
+// columns split over CTAs) and lora_expand (the parts of h joined, y += s B h),
+// the second launched while the first runs.
+//
+// Both are products of a weight tile with a few tokens, bound by reading the
+// weights (few tokens an adapter) or x and y (many): tensor-core tiles whose
+// M is the weights' rows and whose N is the tokens, so that one token wastes
+// only multiplications, and every operand goes from memory straight into the
+// fragment that needs it: the order of K is free, so a lane takes four
+// neighbouring columns where the fragment layout names columns t and t + 4.
+// F16 and BF16 weights are TF32 numbers as they are; x, h and F32 weights go
+// in as two, hi + lo (x.hi, x.lo and, for F32, lo.hi products; 2^-22 of a term
+// is lost at most).  Sums are f32.
+//
+// Tokens of one adapter are gathered into tiles.  A token's sums are made in
+// the same order whatever tile and place it lands in.
 #include <cuda_bf16.h>
 
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -16,7 +30,16 @@ namespace glmvx {
 namespace {
 
 constexpr int kLoraMaxRank = 256;
-constexpr int kLoraThreads = 256;
+constexpr int kLoraThreads = 256, kLoraWarps = kLoraThreads / 32;
+constexpr int kLoraScan = 1024;      // tokens up to which each CTA finds its tile's tokens itself
+constexpr int kLoraMaxSplits = 32;
+constexpr int kLoraRankChunk = 64;   // ranks a shrink CTA takes
+constexpr int kLoraRows = 32;        // rows of B a warp takes at once
+
+// A tile of the plan: n tokens of one adapter, order[start ..].
+struct LoraTile {
+    int adapter, start, n, pad;
+};
 
 struct LoraArgs {
     float *y;
@@ -25,72 +48,431 @@ struct LoraArgs {
     const void *a, *b;
     const int32_t *ranks;
     const float *scales;
-    float *h;
+    float *h;         // [splits][tokens][max_rank]
+    LoraTile *tiles;  // the plan (NULL: CTAs scan the ids)
+    int *order, *counts, *places, *ntiles;
     int64_t y_stride, x_stride;
-    int tokens, rows, cols, adapters, max_rank;
+    int tokens, rows, cols, adapters, max_rank, splits, units, row_steps;
     int *err;
 };
 
-__device__ __forceinline__ float lora_f32(float v) { return v; }
-__device__ __forceinline__ float lora_f32(__half v) { return __half2float(v); }
-__device__ __forceinline__ float lora_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
-
-// The adapter of token t, or -1; an id outside the bank is reported.
-__device__ __forceinline__ int lora_adapter(const LoraArgs &p, int t) {
-    const int a = p.ids[t];
-    if (a < 0) return -1;
-    if (a < p.adapters) return a;
-    if (threadIdx.x == 0) report_device_error(p.err, kDevErrBadIndex);
-    return -1;
-}
-
 __device__ __forceinline__ int lora_rank(const LoraArgs &p, int a) { return min(max(p.ranks[a], 0), p.max_rank); }
 
-// One CTA per token, a warp per row of A.
+// Four neighbouring values as they stand in memory; those from `n` on are 0
+// (n <= 0: nothing is read).
 template <class W>
-__global__ void __launch_bounds__(kLoraThreads) lora_shrink_kernel(LoraArgs p) {
-    const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int id = lora_adapter(p, t);
-    if (id < 0) return;
-    const int rank = lora_rank(p, id);
-    const float *x = p.x + t * p.x_stride;
-    for (int r = warp; r < rank; r += kLoraThreads / 32) {
-        const W *a = static_cast<const W *>(p.a) + (static_cast<int64_t>(id) * p.max_rank + r) * p.cols;
-        float sum = 0.0f;
-        for (int c = lane; c < p.cols; c += 32) sum = fmaf(lora_f32(a[c]), x[c], sum);
-        sum = warp_sum(sum);
-        if (lane == 0) p.h[static_cast<int64_t>(t) * p.max_rank + r] = sum;
+using LoraRaw = std::conditional_t<sizeof(W) == 4, uint4, uint2>;
+
+template <class W, bool VEC>
+__device__ __forceinline__ LoraRaw<W> lora_load4(const W *w, int n) {
+    LoraRaw<W> raw{};
+    if constexpr (VEC) {
+        if (n > 0) raw = __ldg(reinterpret_cast<const LoraRaw<W> *>(w));
+        if (n < 4) {
+            if constexpr (sizeof(W) == 4) {
+                raw.y = n > 1 ? raw.y : 0u, raw.z = n > 2 ? raw.z : 0u, raw.w = 0u;
+            } else {
+                raw.x = n > 1 ? raw.x : raw.x & 0xffffu, raw.y = n > 2 ? raw.y & 0xffffu : 0u;
+            }
+        }
+    } else if constexpr (sizeof(W) == 4) {
+        const uint32_t *v = reinterpret_cast<const uint32_t *>(w);
+        if (n > 0) raw.x = __ldg(v);
+        if (n > 1) raw.y = __ldg(v + 1);
+        if (n > 2) raw.z = __ldg(v + 2);
+        if (n > 3) raw.w = __ldg(v + 3);
+    } else {
+        const uint16_t *v = reinterpret_cast<const uint16_t *>(w);
+        if (n > 0) raw.x = __ldg(v);
+        if (n > 1) raw.x |= static_cast<uint32_t>(__ldg(v + 1)) << 16;
+        if (n > 2) raw.y = __ldg(v + 2);
+        if (n > 3) raw.y |= static_cast<uint32_t>(__ldg(v + 3)) << 16;
+    }
+    return raw;
+}
+
+template <class W>
+__device__ __forceinline__ float4 lora_f32(const LoraRaw<W> &raw) {
+    if constexpr (sizeof(W) == 4) {
+        return make_float4(__uint_as_float(raw.x), __uint_as_float(raw.y), __uint_as_float(raw.z), __uint_as_float(raw.w));
+    } else if constexpr (std::is_same_v<W, __half>) {
+        const float2 lo = __half22float2(*reinterpret_cast<const __half2 *>(&raw.x));
+        const float2 hi = __half22float2(*reinterpret_cast<const __half2 *>(&raw.y));
+        return make_float4(lo.x, lo.y, hi.x, hi.y);
+    } else {
+        return make_float4(__uint_as_float(raw.x << 16), __uint_as_float(raw.x & 0xffff0000u),
+                           __uint_as_float(raw.y << 16), __uint_as_float(raw.y & 0xffff0000u));
     }
 }
 
-// One CTA per token and kLoraThreads rows, a thread per row of B.
-template <class W>
-__global__ void __launch_bounds__(kLoraThreads) lora_expand_kernel(LoraArgs p) {
-    const int t = blockIdx.x, n = blockIdx.y * kLoraThreads + threadIdx.x;
-    const int id = lora_adapter(p, t);
-    if (id < 0 || n >= p.rows) return;
-    const int rank = lora_rank(p, id);
-    if (rank == 0) return;
-    const W *b = static_cast<const W *>(p.b) + (static_cast<int64_t>(id) * p.rows + n) * p.max_rank;
-    const float *h = p.h + static_cast<int64_t>(t) * p.max_rank;
-    float sum = 0.0f;
-    for (int r = 0; r < rank; ++r) sum = fmaf(lora_f32(b[r]), h[r], sum);
-    float *y = p.y + t * p.y_stride + n;
-    *y = fmaf(p.scales[id], sum, *y);
+__device__ __forceinline__ uint32_t lora_tf32(float x) {
+    uint32_t r;
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
+    return r;
 }
 
-template <class W>
-int32_t lora_launch(const LoraArgs &p, cudaStream_t stream) {
-    lora_shrink_kernel<W><<<p.tokens, kLoraThreads, 0, stream>>>(p);
-    if (const int32_t rc = launch_status("lora_shrink_kernel")) return rc;
-    const dim3 grid(p.tokens, (p.rows + kLoraThreads - 1) / kLoraThreads);
-    lora_expand_kernel<W><<<grid, kLoraThreads, 0, stream>>>(p);
+// x = hi + lo, both TF32.
+__device__ __forceinline__ void lora_split(const float4 &x, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+    const float v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        hi[e] = lora_tf32(v[e]);
+        lo[e] = lora_tf32(v[e] - __uint_as_float(hi[e]));
+    }
+}
+
+__device__ __forceinline__ void lora_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// c += W x over 16 columns, four a lane: `top` and `low` are the lane's weights of rows g and
+// g + 8 of the tile (g = lane / 4), hi and lo its token's x.  SPLIT: the weights are not TF32 numbers.
+template <bool SPLIT>
+__device__ __forceinline__ void lora_unit(float (&c)[4], const float4 &top, const float4 &low, const uint32_t (&hi)[4],
+                                          const uint32_t (&lo)[4]) {
+    uint32_t th[4], lh[4];
+    if constexpr (SPLIT) {
+        uint32_t tl[4], ll[4];
+        lora_split(top, th, tl);
+        lora_split(low, lh, ll);
+#pragma unroll
+        for (int s = 0; s < 4; s += 2) lora_mma(c, tl[s], ll[s], tl[s + 1], ll[s + 1], hi[s], hi[s + 1]);
+    } else {
+        th[0] = __float_as_uint(top.x), th[1] = __float_as_uint(top.y);
+        th[2] = __float_as_uint(top.z), th[3] = __float_as_uint(top.w);
+        lh[0] = __float_as_uint(low.x), lh[1] = __float_as_uint(low.y);
+        lh[2] = __float_as_uint(low.z), lh[3] = __float_as_uint(low.w);
+    }
+#pragma unroll
+    for (int s = 0; s < 4; s += 2) lora_mma(c, th[s], lh[s], th[s + 1], lh[s + 1], lo[s], lo[s + 1]);
+#pragma unroll
+    for (int s = 0; s < 4; s += 2) lora_mma(c, th[s], lh[s], th[s + 1], lh[s + 1], hi[s], hi[s + 1]);
+}
+
+// The tile of this CTA (blockIdx.x): its adapter (-1: no tile), its tokens and their number.  With a
+// plan it is the plan's.  Without, CTA t leads a tile if token t is the first, or
+// TILE-th, 2 TILE-th ..., of its adapter's tokens; the tile is t and the next ones.
+template <int TILE>
+__device__ __forceinline__ int lora_tile(const LoraArgs &p, int (&tokens)[TILE], int &n, bool report) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, t = blockIdx.x;
+    if (p.tiles) {
+        if (t >= *p.ntiles) return -1;
+        const LoraTile tile = p.tiles[t];
+        for (int i = tid; i < tile.n; i += kLoraThreads) tokens[i] = p.order[tile.start + i];
+        if (tid == 0) n = tile.n;
+        __syncthreads();
+        return tile.adapter;
+    }
+    __shared__ uint32_t match[kLoraScan / 32];
+    const int a = p.ids[t];
+    if (a >= p.adapters && report && tid == 0) report_device_error(p.err, kDevErrBadIndex);
+    if (a < 0 || a >= p.adapters) return -1;
+    const int words = (p.tokens + 31) / 32;
+    for (int w = warp; w < words; w += kLoraWarps) {
+        const int j = 32 * w + lane;
+        const uint32_t m = __ballot_sync(0xffffffffu, j < p.tokens && p.ids[j] == a);
+        if (lane == 0) match[w] = m;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        const uint32_t m = lane < words ? match[lane] : 0u;
+        const int mine = __popc(m);
+        int before = mine;  // matches in the words before this lane's
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, before, o);
+            if (lane >= o) before += up;
+        }
+        const int all = __shfl_sync(0xffffffffu, before, 31);
+        before -= mine;
+        const int lead = __shfl_sync(0xffffffffu, before + __popc(m & ((1u << (t & 31)) - 1)), t >> 5);
+        const int here = lead % TILE ? 0 : min(TILE, all - lead);
+        if (here)
+            for (uint32_t left = m, r = before; left; left &= left - 1, ++r) {
+                const int at = static_cast<int>(r) - lead;
+                if (at >= 0 && at < here) tokens[at] = 32 * lane + __ffs(left) - 1;
+            }
+        if (lane == 0) n = here;
+    }
+    __syncthreads();
+    return n ? a : -1;
+}
+
+// Tiles of up to `tile` tokens of one adapter: one CTA counts the adapters'
+// tokens, gives each adapter its place in the order, and lists the tiles.  The
+// order within an adapter is that of the atomics, which no result depends on.
+constexpr int kLoraPlanThreads = 1024;
+__global__ void __launch_bounds__(kLoraPlanThreads) lora_plan_kernel(LoraArgs p, int tile) {
+    __shared__ int warp_tokens[32], warp_tiles[32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    for (int a = tid; a < p.adapters; a += kLoraPlanThreads) p.counts[a] = 0;
+    __syncthreads();
+    for (int t = tid; t < p.tokens; t += kLoraPlanThreads) {
+        const int a = p.ids[t];
+        if (a >= p.adapters) report_device_error(p.err, kDevErrBadIndex);
+        p.places[t] = a >= 0 && a < p.adapters ? atomicAdd(p.counts + a, 1) : 0;
+    }
+    __syncthreads();
+    int token_base = 0, tile_base = 0;  // of the adapters before this round's
+    for (int a0 = 0; a0 < p.adapters; a0 += kLoraPlanThreads) {
+        const int a = a0 + tid, n = a < p.adapters ? p.counts[a] : 0, nt = (n + tile - 1) / tile;
+        int sn = n, st = nt;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int un = __shfl_up_sync(0xffffffffu, sn, o), ut = __shfl_up_sync(0xffffffffu, st, o);
+            if (lane >= o) sn += un, st += ut;
+        }
+        if (lane == 31) warp_tokens[warp] = sn, warp_tiles[warp] = st;
+        __syncthreads();
+        int start = token_base + sn - n, first = tile_base + st - nt;
+        for (int w = 0; w < kLoraPlanThreads / 32; ++w) {
+            if (w < warp) start += warp_tokens[w], first += warp_tiles[w];
+            token_base += warp_tokens[w], tile_base += warp_tiles[w];
+        }
+        if (a < p.adapters) p.counts[a] = start;
+        for (int i = 0; i < nt; ++i) p.tiles[first + i] = {a, start + i * tile, min(tile, n - i * tile), 0};
+        __syncthreads();
+    }
+    for (int t = tid; t < p.tokens; t += kLoraPlanThreads) {
+        const int a = p.ids[t];
+        if (a >= 0 && a < p.adapters) p.order[p.counts[a] + p.places[t]] = t;
+    }
+    if (tid == 0) *p.ntiles = tile_base;
+}
+
+// h[split][token][r] = A[r][the split's columns] . x[token][the split's columns]
+// for a tile of 8 NT tokens and 16 MT MW ranks (blockIdx.z: which).  MW warps
+// share a unit of 16 columns, 16 MT ranks each, and take every 8 / MW-th unit, kUnits
+// of them in flight; the warps' sums are joined in order.
+template <class W, int MT, int MW, int NT, bool VEC>
+__global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(LoraArgs p) {
+    constexpr int kUnits = NT == 1 ? 4 : 2, kKWarps = kLoraWarps / MW, kRanks = 16 * MT * MW, kStride = 8 * NT + 1;
+    __shared__ int tokens[8 * NT], n;
+    __shared__ float parts[kKWarps][kRanks * kStride];
+    allow_dependent_launch();
+    const int a = lora_tile<8 * NT>(p, tokens, n, blockIdx.y == 0 && blockIdx.z == 0);
+    if (a < 0) return;
+    const int rank = lora_rank(p, a), r0 = blockIdx.z * kRanks;
+    if (r0 >= rank) return;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = 4 * (lane & 3);
+    const int kw = warp / MW, rw = r0 + 16 * MT * (warp % MW) + g;  // the lane's first rank
+    const int split = blockIdx.y, u0 = split * p.units, u1 = min(u0 + p.units, (p.cols + 15) / 16);
+    const W *w = static_cast<const W *>(p.a) + (static_cast<int64_t>(a) * p.max_rank + rw) * p.cols;
+    const float *x[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) x[j] = 8 * j + g < n ? p.x + tokens[8 * j + g] * p.x_stride : nullptr;
+    float acc[MT][NT][4] = {};
+    for (int u = u0 + kw; u < u1; u += kUnits * kKWarps) {
+        LoraRaw<W> wt[kUnits][MT][2];
+        uint4 xv[kUnits][NT];
+#pragma unroll
+        for (int k = 0; k < kUnits; ++k) {
+            const int c = 16 * (u + k * kKWarps) + t4, left = u + k * kKWarps < u1 ? p.cols - c : 0;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) xv[k][j] = lora_load4<float, VEC>(x[j] + c, x[j] ? left : 0);
+#pragma unroll
+            for (int i = 0; i < 2 * MT; ++i)
+                wt[k][i / 2][i % 2] =
+                    lora_load4<W, VEC>(w + static_cast<int64_t>(8 * i) * p.cols + c, rw + 8 * i < rank ? left : 0);
+        }
+#pragma unroll
+        for (int k = 0; k < kUnits; ++k) {
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                uint32_t hi[4], lo[4];
+                lora_split(lora_f32<float>(xv[k][j]), hi, lo);
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+                    lora_unit<sizeof(W) == 4>(acc[i][j], lora_f32<W>(wt[k][i][0]), lora_f32<W>(wt[k][i][1]), hi, lo);
+            }
+        }
+    }
+    // acc[i][j]: ranks rw + 16 i (+ 8), tokens 8 j + t4 / 2 (+ 1)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            float *at = parts[kw] + (rw - r0 + 16 * i) * kStride + 8 * j + t4 / 2;
+            at[0] = acc[i][j][0], at[1] = acc[i][j][1];
+            at[8 * kStride] = acc[i][j][2], at[8 * kStride + 1] = acc[i][j][3];
+        }
+    }
+    __syncthreads();
+    const int ranks = min(kRanks, rank - r0);
+    for (int i = tid; i < n * kRanks; i += kLoraThreads) {
+        const int tok = i / kRanks, r = i % kRanks;
+        if (r >= ranks) continue;
+        float sum = 0.0f;
+#pragma unroll
+        for (int v = 0; v < kKWarps; ++v) sum += parts[v][r * kStride + tok];
+        p.h[(static_cast<int64_t>(split) * p.tokens + tokens[tok]) * p.max_rank + r0 + r] = sum;
+    }
+}
+
+// y[token][row] += s * B[row] . h[token] for a tile of 8 NT tokens; blockIdx.y takes
+// row_steps groups of 32 rows per warp.  Row 4 g + i of a warp's 32 stands at
+// place g of half i of two m16 tiles, so that a lane ends up with four
+// neighbouring rows of two tokens: one float4 of y each.
+template <class W, int NT, bool VEC>
+__global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(LoraArgs p) {
+    extern __shared__ __align__(16) float hs[];  // [2][8 NT][stride]: hi, lo
+    __shared__ int tokens[8 * NT], n;
+    const int a = lora_tile<8 * NT>(p, tokens, n, false);
+    if (a < 0) return;
+    const int rank = lora_rank(p, a), units = (rank + 15) / 16, stride = 16 * units + 4;
+    if (rank == 0) return;
+    const float scale = p.scales[a];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = 4 * (lane & 3);
+    float *ls = hs + 8 * NT * stride;
+    grid_dependency_wait();  // h comes from the kernel before
+    for (int i = tid; i < 8 * NT * 16 * units; i += kLoraThreads) {
+        const int tok = i / (16 * units), r = i - tok * 16 * units;
+        float sum = 0.0f;
+        if (tok < n && r < rank) {
+            const float *h = p.h + static_cast<int64_t>(tokens[tok]) * p.max_rank + r;
+            for (int s = 0; s < p.splits; ++s) sum += h[static_cast<int64_t>(s) * p.tokens * p.max_rank];
+        }
+        const uint32_t hi = lora_tf32(sum);
+        hs[tok * stride + r] = __uint_as_float(hi);
+        ls[tok * stride + r] = __uint_as_float(lora_tf32(sum - __uint_as_float(hi)));
+    }
+    __syncthreads();
+    const W *b = static_cast<const W *>(p.b) + static_cast<int64_t>(a) * p.rows * p.max_rank;
+    for (int step = 0; step < p.row_steps; ++step) {
+        const int row = ((blockIdx.y * p.row_steps + step) * kLoraWarps + warp) * kLoraRows + 4 * g;
+        if (row - 4 * g >= p.rows) break;
+        uint4 old[NT][2];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int tok = 8 * j + t4 / 2 + e;
+                old[j][e] = lora_load4<float, VEC>(tok < n ? p.y + tokens[tok] * p.y_stride + row : nullptr,
+                                                   tok < n ? p.rows - row : 0);
+            }
+        }
+        float acc[2][NT][4] = {};
+        for (int u = 0; u < units; ++u) {
+            const int r = 16 * u + t4;
+            LoraRaw<W> wt[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                wt[i] = lora_load4<W, VEC>(b + static_cast<int64_t>(row + i) * p.max_rank + r,
+                                           row + i < p.rows ? rank - r : 0);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const int at = (8 * j + g) * stride + r;
+                const uint4 h4 = *reinterpret_cast<const uint4 *>(hs + at), l4 = *reinterpret_cast<const uint4 *>(ls + at);
+                const uint32_t hi[4] = {h4.x, h4.y, h4.z, h4.w}, lo[4] = {l4.x, l4.y, l4.z, l4.w};
+                lora_unit<sizeof(W) == 4>(acc[0][j], lora_f32<W>(wt[0]), lora_f32<W>(wt[1]), hi, lo);
+                lora_unit<sizeof(W) == 4>(acc[1][j], lora_f32<W>(wt[2]), lora_f32<W>(wt[3]), hi, lo);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int tok = 8 * j + t4 / 2 + e;
+                if (tok >= n || row >= p.rows) continue;
+                const float4 o = lora_f32<float>(old[j][e]);
+                const float v[4] = {fmaf(scale, acc[0][j][e], o.x), fmaf(scale, acc[0][j][2 + e], o.y),
+                                    fmaf(scale, acc[1][j][e], o.z), fmaf(scale, acc[1][j][2 + e], o.w)};
+                float *y = p.y + tokens[tok] * p.y_stride + row;
+                if (VEC) {
+                    *reinterpret_cast<float4 *>(y) = make_float4(v[0], v[1], v[2], v[3]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (row + i < p.rows) y[i] = v[i];
+                }
+            }
+        }
+    }
+}
+
+constexpr int lora_ceil(int64_t n, int64_t of) { return static_cast<int>((n + of - 1) / of); }
+
+// Parts that the columns are cut into, at most: enough CTAs for few tokens.
+int lora_max_splits(int tokens) { return std::clamp(lora_ceil(16384, tokens), 1, kLoraMaxSplits); }
+
+// The workspace: h, then (where there is a plan) the tiles, the order, the places, the counts.
+struct LoraLayout {
+    int64_t tiles, order, places, counts, ntiles, bytes;
+};
+LoraLayout lora_layout(int64_t tokens, int64_t adapters, int64_t max_rank) {
+    LoraLayout l{};
+    tokens = std::max<int64_t>(tokens, 1);
+    const auto take = [&](int64_t n) {
+        const int64_t at = l.bytes;
+        l.bytes += (n + 15) & ~int64_t{15};
+        return at;
+    };
+    take(4 * tokens * max_rank * lora_max_splits(static_cast<int>(tokens)));
+    if (tokens > kLoraScan) {
+        l.tiles = take(sizeof(LoraTile) * tokens);
+        l.order = take(4 * tokens);
+        l.places = take(4 * tokens);
+        l.counts = take(4 * adapters);
+        l.ntiles = take(4);
+    }
+    return l;
+}
+
+template <class W, int MT, int MW, int NT>
+int32_t lora_shrink(const LoraArgs &p, dim3 grid, bool vec, cudaStream_t stream) {
+    if (vec) lora_shrink_kernel<W, MT, MW, NT, true><<<grid, kLoraThreads, 0, stream>>>(p);
+    else lora_shrink_kernel<W, MT, MW, NT, false><<<grid, kLoraThreads, 0, stream>>>(p);
+    return launch_status("lora_shrink_kernel");
+}
+
+template <class W, int NT, bool VEC>
+int32_t lora_expand(const LoraArgs &p, dim3 grid, cudaStream_t stream) {
+    const size_t smem = sizeof(float) * 2 * 8 * NT * (16 * lora_ceil(p.max_rank, 16) + 4);
+    if (const int32_t rc = allow_dynamic_smem(lora_expand_kernel<W, NT, VEC>, smem, "lora_expand smem")) return rc;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(kLoraThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    GLMVX_CUDA(cudaLaunchKernelEx(&cfg, lora_expand_kernel<W, NT, VEC>, p));
     return launch_status("lora_expand_kernel");
 }
 
-int64_t lora_bytes(int64_t tokens, int64_t adapters, int64_t max_rank) {
-    (void)adapters;
-    return 4 * std::max<int64_t>(tokens, 1) * max_rank;
+template <class W, int NT>
+int32_t lora_launch(LoraArgs &p, bool vec_a, bool vec_b, cudaStream_t stream) {
+    const int sms = sm_count();
+    // CTAs along the tokens: every token may lead a tile, or the plan's most.
+    const int tiles = p.tiles ? static_cast<int>(std::min<int64_t>(p.tokens, p.tokens / (8 * NT) + int64_t{p.adapters}))
+                              : p.tokens;
+    if (p.tiles) {
+        lora_plan_kernel<<<1, kLoraPlanThreads, 0, stream>>>(p, 8 * NT);
+        if (const int32_t rc = launch_status("lora_plan_kernel")) return rc;
+    }
+    // Columns in as many parts as give four CTAs an SM, none shorter than four units a warp.
+    const int full = lora_ceil(p.tokens, 8 * NT), all_units = lora_ceil(p.cols, 16);
+    p.splits = std::min({lora_max_splits(p.tokens), lora_ceil(all_units, 4 * kLoraWarps), lora_ceil(4 * sms, full)});
+    p.units = lora_ceil(all_units, p.splits);
+    p.splits = lora_ceil(all_units, p.units);
+    const int ranks = p.max_rank <= 16 ? 16 : p.max_rank <= 32 ? 32 : kLoraRankChunk;
+    const dim3 grid(tiles, p.splits, lora_ceil(p.max_rank, ranks));
+    int32_t rc = kOk;
+    if (ranks == 16) rc = lora_shrink<W, 1, 1, NT>(p, grid, vec_a, stream);
+    else if (ranks == 32) rc = lora_shrink<W, 2, 1, NT>(p, grid, vec_a, stream);
+    else rc = lora_shrink<W, 2, 2, NT>(p, grid, vec_a, stream);
+    if (rc) return rc;
+    const int steps = lora_ceil(p.rows, kLoraWarps * kLoraRows);
+    p.row_steps = std::max(1, static_cast<int>(int64_t{steps} * full / (8 * sms)));
+    const dim3 out(tiles, lora_ceil(steps, p.row_steps));
+    return vec_b ? lora_expand<W, NT, true>(p, out, stream) : lora_expand<W, NT, false>(p, out, stream);
 }
 
 }  // namespace
@@ -101,7 +483,7 @@ using namespace glmvx;
 
 GLMVX_EXPORT int64_t glmvx_lora_workspace_bytes(int32_t tokens, int32_t adapters, int32_t max_rank) {
     if (tokens < 0 || tokens > 1 << 20 || adapters < 1 || max_rank < 1 || max_rank > kLoraMaxRank) return kInvalid;
-    return lora_bytes(tokens, adapters, max_rank);
+    return lora_layout(tokens, adapters, max_rank).bytes;
 }
 
 GLMVX_EXPORT int32_t glmvx_lora_add(float *y, int64_t y_stride, const float *x, int64_t x_stride,
@@ -124,12 +506,31 @@ GLMVX_EXPORT int32_t glmvx_lora_add(float *y, int64_t y_stride, const float *x, 
     if (((bits(y) | bits(x) | bits(adapter_ids) | bits(ranks) | bits(scales)) & 3) || (bits(workspace) & 15) ||
         ((bits(a) | bits(b)) & (kind == 0 ? 3 : 1)))
         return set_error("lora_add: misaligned pointer"), kInvalid;
-    if (workspace_bytes < static_cast<uint64_t>(lora_bytes(tokens, adapters, max_rank)))
+    const LoraLayout layout = lora_layout(tokens, adapters, max_rank);
+    if (workspace_bytes < static_cast<uint64_t>(layout.bytes))
         return set_error("lora_add: workspace smaller than glmvx_lora_workspace_bytes"), kInvalid;
-    const LoraArgs p{y, x, adapter_ids, a, b, ranks, scales, static_cast<float *>(workspace), y_stride, x_stride,
-                     tokens, rows, cols, adapters, max_rank, device_error_word()};
+    LoraArgs p{};
+    p.y = y, p.x = x, p.ids = adapter_ids, p.a = a, p.b = b, p.ranks = ranks, p.scales = scales;
+    p.y_stride = y_stride, p.x_stride = x_stride;
+    p.tokens = tokens, p.rows = rows, p.cols = cols, p.adapters = adapters, p.max_rank = max_rank;
+    p.err = device_error_word();
+    uint8_t *ws = static_cast<uint8_t *>(workspace);
+    p.h = reinterpret_cast<float *>(ws);
+    if (tokens > kLoraScan) {
+        p.tiles = reinterpret_cast<LoraTile *>(ws + layout.tiles);
+        p.order = reinterpret_cast<int *>(ws + layout.order);
+        p.places = reinterpret_cast<int *>(ws + layout.places);
+        p.counts = reinterpret_cast<int *>(ws + layout.counts);
+        p.ntiles = reinterpret_cast<int *>(ws + layout.ntiles);
+    }
+    // Four neighbours at once where they stand on their boundary.
+    const int four = kind == 0 ? 15 : 7;
+    const bool vec_a = !(cols & 3) && !(bits(a) & four) && !(bits(x) & 15) && (tokens == 1 || !(x_stride & 3));
+    const bool vec_b = !(max_rank & 3) && !(rows & 3) && !(bits(b) & four) && !(bits(y) & 15) &&
+                       (tokens == 1 || !(y_stride & 3));
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (kind == 0) return lora_launch<float>(p, s);
-    if (kind == 1) return lora_launch<__half>(p, s);
-    return lora_launch<__nv_bfloat16>(p, s);
+    const bool wide = tokens > 64;
+    if (kind == 0) return wide ? lora_launch<float, 4>(p, vec_a, vec_b, s) : lora_launch<float, 1>(p, vec_a, vec_b, s);
+    if (kind == 1) return wide ? lora_launch<__half, 4>(p, vec_a, vec_b, s) : lora_launch<__half, 1>(p, vec_a, vec_b, s);
+    return wide ? lora_launch<__nv_bfloat16, 4>(p, vec_a, vec_b, s) : lora_launch<__nv_bfloat16, 1>(p, vec_a, vec_b, s);
 }
