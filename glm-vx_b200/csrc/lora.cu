@@ -31,7 +31,7 @@ namespace {
 
 constexpr int kLoraMaxRank = 256;
 constexpr int kLoraThreads = 256, kLoraWarps = kLoraThreads / 32;
-constexpr int kLoraScan = 1024;      // tokens up to which each CTA finds its tile's tokens itself
+constexpr int kLoraScan = 64;        // tokens up to which each CTA finds its tile's tokens itself
 constexpr int kLoraMaxSplits = 32;
 constexpr int kLoraRankChunk = 64;   // ranks a shrink CTA takes
 constexpr int kLoraRows = 32;        // rows of B a warp takes at once
@@ -59,7 +59,7 @@ struct LoraArgs {
 __device__ __forceinline__ int lora_rank(const LoraArgs &p, int a) { return min(max(p.ranks[a], 0), p.max_rank); }
 
 // Four neighbouring values as they stand in memory; those from `n` on are 0
-// (n <= 0: nothing is read).
+// (n <= 0: nothing is read).  With VEC n is never 1 to 3.
 template <class W>
 using LoraRaw = std::conditional_t<sizeof(W) == 4, uint4, uint2>;
 
@@ -68,13 +68,6 @@ __device__ __forceinline__ LoraRaw<W> lora_load4(const W *w, int n) {
     LoraRaw<W> raw{};
     if constexpr (VEC) {
         if (n > 0) raw = __ldg(reinterpret_cast<const LoraRaw<W> *>(w));
-        if (n < 4) {
-            if constexpr (sizeof(W) == 4) {
-                raw.y = n > 1 ? raw.y : 0u, raw.z = n > 2 ? raw.z : 0u, raw.w = 0u;
-            } else {
-                raw.x = n > 1 ? raw.x : raw.x & 0xffffu, raw.y = n > 2 ? raw.y & 0xffffu : 0u;
-            }
-        }
     } else if constexpr (sizeof(W) == 4) {
         const uint32_t *v = reinterpret_cast<const uint32_t *>(w);
         if (n > 0) raw.x = __ldg(v);
@@ -89,6 +82,21 @@ __device__ __forceinline__ LoraRaw<W> lora_load4(const W *w, int n) {
         if (n > 3) raw.y |= static_cast<uint32_t>(__ldg(v + 3)) << 16;
     }
     return raw;
+}
+
+// Keeps the first n of the four values (n <= 0: none).
+template <class W>
+__device__ __forceinline__ LoraRaw<W> lora_mask(int n) {
+    if constexpr (sizeof(W) == 4) {
+        return make_uint4(n > 0 ? ~0u : 0u, n > 1 ? ~0u : 0u, n > 2 ? ~0u : 0u, n > 3 ? ~0u : 0u);
+    } else {
+        return make_uint2(n > 1 ? ~0u : n > 0 ? 0xffffu : 0u, n > 3 ? ~0u : n > 2 ? 0xffffu : 0u);
+    }
+}
+
+__device__ __forceinline__ void lora_keep(uint2 &raw, const uint2 &mask) { raw.x &= mask.x, raw.y &= mask.y; }
+__device__ __forceinline__ void lora_keep(uint4 &raw, const uint4 &mask) {
+    raw.x &= mask.x, raw.y &= mask.y, raw.z &= mask.z, raw.w &= mask.w;
 }
 
 template <class W>
@@ -203,23 +211,35 @@ __device__ __forceinline__ int lora_tile(const LoraArgs &p, int (&tokens)[TILE],
 }
 
 // Tiles of up to `tile` tokens of one adapter: one CTA counts the adapters'
-// tokens, gives each adapter its place in the order, and lists the tiles.  The
-// order within an adapter is that of the atomics, which no result depends on.
-constexpr int kLoraPlanThreads = 1024;
+// tokens (in shared memory when the adapters fit), gives each adapter its place
+// in the order, and lists the tiles.  The order within an adapter is that of
+// the atomics, which no result depends on.
+constexpr int kLoraPlanThreads = 1024, kLoraPlanOwn = 4, kLoraPlanCounts = 4096;
 __global__ void __launch_bounds__(kLoraPlanThreads) lora_plan_kernel(LoraArgs p, int tile) {
-    __shared__ int warp_tokens[32], warp_tiles[32];
+    __shared__ int warp_tokens[32], warp_tiles[32], near_counts[kLoraPlanCounts];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    for (int a = tid; a < p.adapters; a += kLoraPlanThreads) p.counts[a] = 0;
+    allow_dependent_launch();
+    int *counts = p.adapters <= kLoraPlanCounts ? near_counts : p.counts;
+    for (int a = tid; a < p.adapters; a += kLoraPlanThreads) counts[a] = 0;
+    int own[kLoraPlanOwn], place[kLoraPlanOwn];  // the thread's first tokens
+#pragma unroll
+    for (int k = 0; k < kLoraPlanOwn; ++k) {
+        const int t = tid + k * kLoraPlanThreads, a = t < p.tokens ? p.ids[t] : -1;
+        if (a >= p.adapters) report_device_error(p.err, kDevErrBadIndex);
+        own[k] = a < p.adapters ? a : -1;
+    }
     __syncthreads();
-    for (int t = tid; t < p.tokens; t += kLoraPlanThreads) {
+#pragma unroll
+    for (int k = 0; k < kLoraPlanOwn; ++k) place[k] = own[k] >= 0 ? atomicAdd(counts + own[k], 1) : 0;
+    for (int t = tid + kLoraPlanOwn * kLoraPlanThreads; t < p.tokens; t += kLoraPlanThreads) {
         const int a = p.ids[t];
         if (a >= p.adapters) report_device_error(p.err, kDevErrBadIndex);
-        p.places[t] = a >= 0 && a < p.adapters ? atomicAdd(p.counts + a, 1) : 0;
+        p.places[t] = a >= 0 && a < p.adapters ? atomicAdd(counts + a, 1) : 0;
     }
     __syncthreads();
     int token_base = 0, tile_base = 0;  // of the adapters before this round's
     for (int a0 = 0; a0 < p.adapters; a0 += kLoraPlanThreads) {
-        const int a = a0 + tid, n = a < p.adapters ? p.counts[a] : 0, nt = (n + tile - 1) / tile;
+        const int a = a0 + tid, n = a < p.adapters ? counts[a] : 0, nt = (n + tile - 1) / tile;
         int sn = n, st = nt;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -233,26 +253,33 @@ __global__ void __launch_bounds__(kLoraPlanThreads) lora_plan_kernel(LoraArgs p,
             if (w < warp) start += warp_tokens[w], first += warp_tiles[w];
             token_base += warp_tokens[w], tile_base += warp_tiles[w];
         }
-        if (a < p.adapters) p.counts[a] = start;
+        if (a < p.adapters) counts[a] = start;
         for (int i = 0; i < nt; ++i) p.tiles[first + i] = {a, start + i * tile, min(tile, n - i * tile), 0};
         __syncthreads();
     }
-    for (int t = tid; t < p.tokens; t += kLoraPlanThreads) {
+#pragma unroll
+    for (int k = 0; k < kLoraPlanOwn; ++k)
+        if (own[k] >= 0) p.order[counts[own[k]] + place[k]] = tid + k * kLoraPlanThreads;
+    for (int t = tid + kLoraPlanOwn * kLoraPlanThreads; t < p.tokens; t += kLoraPlanThreads) {
         const int a = p.ids[t];
-        if (a >= 0 && a < p.adapters) p.order[p.counts[a] + p.places[t]] = t;
+        if (a >= 0 && a < p.adapters) p.order[counts[a] + p.places[t]] = t;
     }
     if (tid == 0) *p.ntiles = tile_base;
 }
 
 // h[split][token][r] = A[r][the split's columns] . x[token][the split's columns]
 // for a tile of 8 NT tokens and 16 MT MW ranks (blockIdx.z: which).  MW warps
-// share a unit of 16 columns, 16 MT ranks each, and take every 8 / MW-th unit, kUnits
-// of them in flight; the warps' sums are joined in order.
+// share a unit of 16 columns, 16 MT ranks each, and take every 8 / MW-th unit, two
+// at a time, the next two on their way meanwhile; the warps' sums are joined in
+// order.  Lanes without a token or a rank of their own read the first one's:
+// what they make is a column or a row of the tile that nobody keeps.
 template <class W, int MT, int MW, int NT, bool VEC>
 __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(LoraArgs p) {
-    constexpr int kUnits = NT == 1 ? 4 : 2, kKWarps = kLoraWarps / MW, kRanks = 16 * MT * MW, kStride = 8 * NT + 1;
+    constexpr int kUnits = 2, kKWarps = kLoraWarps / MW, kRanks = 16 * MT * MW, kStride = 8 * NT + 1;
+    constexpr int kStep = 16 * kKWarps;  // columns from a warp's unit to its next
     __shared__ int tokens[8 * NT], n;
     __shared__ float parts[kKWarps][kRanks * kStride];
+    grid_dependency_wait();  // the plan comes from the kernel before
     allow_dependent_launch();
     const int a = lora_tile<8 * NT>(p, tokens, n, blockIdx.y == 0 && blockIdx.z == 0);
     if (a < 0) return;
@@ -260,36 +287,60 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(LoraArgs p
     if (r0 >= rank) return;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = 4 * (lane & 3);
     const int kw = warp / MW, rw = r0 + 16 * MT * (warp % MW) + g;  // the lane's first rank
-    const int split = blockIdx.y, u0 = split * p.units, u1 = min(u0 + p.units, (p.cols + 15) / 16);
-    const W *w = static_cast<const W *>(p.a) + (static_cast<int64_t>(a) * p.max_rank + rw) * p.cols;
+    const int split = blockIdx.y, u0 = split * p.units + kw, u1 = min((split + 1) * p.units, (p.cols + 15) / 16);
+    const W *w[2 * MT];
     const float *x[NT];
 #pragma unroll
-    for (int j = 0; j < NT; ++j) x[j] = 8 * j + g < n ? p.x + tokens[8 * j + g] * p.x_stride : nullptr;
+    for (int i = 0; i < 2 * MT; ++i) {
+        const int r = rw + 8 * i < rank ? rw + 8 * i : 0;
+        w[i] = static_cast<const W *>(p.a) + (static_cast<int64_t>(a) * p.max_rank + r) * p.cols + 16 * u0 + t4;
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j) x[j] = p.x + tokens[8 * j + g < n ? 8 * j + g : 0] * p.x_stride + 16 * u0 + t4;
     float acc[MT][NT][4] = {};
-    for (int u = u0 + kw; u < u1; u += kUnits * kKWarps) {
-        LoraRaw<W> wt[kUnits][MT][2];
-        uint4 xv[kUnits][NT];
+    struct Batch {
+        LoraRaw<W> w[kUnits][2 * MT];
+        uint4 x[kUnits][NT];
+    };
+    const auto load = [&](Batch &t, int left) {  // left: columns from the lane's first to the end of the split
 #pragma unroll
         for (int k = 0; k < kUnits; ++k) {
-            const int c = 16 * (u + k * kKWarps) + t4, left = u + k * kKWarps < u1 ? p.cols - c : 0;
 #pragma unroll
-            for (int j = 0; j < NT; ++j) xv[k][j] = lora_load4<float, VEC>(x[j] + c, x[j] ? left : 0);
+            for (int j = 0; j < NT; ++j) t.x[k][j] = lora_load4<float, VEC>(x[j] + k * kStep, left - k * kStep);
 #pragma unroll
-            for (int i = 0; i < 2 * MT; ++i)
-                wt[k][i / 2][i % 2] =
-                    lora_load4<W, VEC>(w + static_cast<int64_t>(8 * i) * p.cols + c, rw + 8 * i < rank ? left : 0);
+            for (int i = 0; i < 2 * MT; ++i) t.w[k][i] = lora_load4<W, VEC>(w[i] + k * kStep, left - k * kStep);
         }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) x[j] += kUnits * kStep;
+#pragma unroll
+        for (int i = 0; i < 2 * MT; ++i) w[i] += kUnits * kStep;
+    };
+    const auto multiply = [&](const Batch &t) {
 #pragma unroll
         for (int k = 0; k < kUnits; ++k) {
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
                 uint32_t hi[4], lo[4];
-                lora_split(lora_f32<float>(xv[k][j]), hi, lo);
+                lora_split(lora_f32<float>(t.x[k][j]), hi, lo);
 #pragma unroll
                 for (int i = 0; i < MT; ++i)
-                    lora_unit<sizeof(W) == 4>(acc[i][j], lora_f32<W>(wt[k][i][0]), lora_f32<W>(wt[k][i][1]), hi, lo);
+                    lora_unit<sizeof(W) == 4>(acc[i][j], lora_f32<W>(t.w[k][2 * i]), lora_f32<W>(t.w[k][2 * i + 1]), hi,
+                                              lo);
             }
         }
+    };
+    Batch even, odd;
+    int left = min(p.cols, 16 * u1) - (16 * u0 + t4);
+    constexpr int kBatch = kUnits * kStep;
+    // left + t4 is what the warp's first lane has left: the same in all lanes
+    load(even, left);
+    while (left + t4 > 0) {
+        if (left + t4 > kBatch) load(odd, left - kBatch);
+        multiply(even);
+        if (left + t4 <= kBatch) break;
+        left -= 2 * kBatch;
+        if (left + t4 > 0) load(even, left);
+        multiply(odd);
     }
     // acc[i][j]: ranks rw + 16 i (+ 8), tokens 8 j + t4 / 2 (+ 1)
 #pragma unroll
@@ -314,16 +365,17 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(LoraArgs p
 }
 
 // y[token][row] += s * B[row] . h[token] for a tile of 8 NT tokens; blockIdx.y takes
-// row_steps groups of 32 rows per warp.  Row 4 g + i of a warp's 32 stands at
-// place g of half i of two m16 tiles, so that a lane ends up with four
-// neighbouring rows of two tokens: one float4 of y each.
-template <class W, int NT, bool VEC>
-__global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(LoraArgs p) {
+// row_steps groups of 32 RG rows per warp.  Row 4 g + i of 32 stands at place
+// g of half i of two m16 tiles, so that a lane ends up with four neighbouring
+// rows of two tokens: one float4 of y each.  KU units of 16 ranks are read at once.
+template <class W, int NT, int RG, int KU, bool VEC>
+__global__ void __launch_bounds__(kLoraThreads, sizeof(W) == 4 ? 2 : 3) lora_expand_kernel(LoraArgs p) {
     extern __shared__ __align__(16) float hs[];  // [2][8 NT][stride]: hi, lo
     __shared__ int tokens[8 * NT], n;
     const int a = lora_tile<8 * NT>(p, tokens, n, false);
     if (a < 0) return;
-    const int rank = lora_rank(p, a), units = (rank + 15) / 16, stride = 16 * units + 4;
+    const int rank = lora_rank(p, a), units = (rank + 15) / 16;
+    const int stride = 16 * (units | 1);  // 16 mod 32 banks: the quarters of a warp's 16-byte reads do not meet
     if (rank == 0) return;
     const float scale = p.scales[a];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = 4 * (lane & 3);
@@ -334,63 +386,120 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(LoraArgs p
         float sum = 0.0f;
         if (tok < n && r < rank) {
             const float *h = p.h + static_cast<int64_t>(tokens[tok]) * p.max_rank + r;
-            for (int s = 0; s < p.splits; ++s) sum += h[static_cast<int64_t>(s) * p.tokens * p.max_rank];
+            const int64_t next = static_cast<int64_t>(p.tokens) * p.max_rank;
+            for (int s = 0; s < p.splits; s += 8) {  // in order, eight in flight
+                float part[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) part[k] = s + k < p.splits ? h[(s + k) * next] : 0.0f;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) sum += part[k];
+            }
         }
         const uint32_t hi = lora_tf32(sum);
         hs[tok * stride + r] = __uint_as_float(hi);
         ls[tok * stride + r] = __uint_as_float(lora_tf32(sum - __uint_as_float(hi)));
     }
     __syncthreads();
-    const W *b = static_cast<const W *>(p.b) + static_cast<int64_t>(a) * p.rows * p.max_rank;
-    for (int step = 0; step < p.row_steps; ++step) {
-        const int row = ((blockIdx.y * p.row_steps + step) * kLoraWarps + warp) * kLoraRows + 4 * g;
-        if (row - 4 * g >= p.rows) break;
-        uint4 old[NT][2];
+    // The lane's rows of B, and its tokens' rows of y from the warp's first row on; a lane without a
+    // token has the first one's, which it reads and does not write.
+    constexpr int kSpan = kLoraRows * RG;
+    const int row_first = (blockIdx.y * p.row_steps * kLoraWarps + warp) * kSpan;
+    const int row_end = min(p.rows, row_first + (p.row_steps - 1) * kLoraWarps * kSpan + kSpan);
+    const W *wr = static_cast<const W *>(p.b) + (static_cast<int64_t>(a) * p.rows + row_first + 4 * g) * p.max_rank + t4;
+    float *y[NT][2];
+    bool mine[NT][2];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
+    for (int j = 0; j < NT; ++j) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int tok = 8 * j + t4 / 2 + e;
-                old[j][e] = lora_load4<float, VEC>(tok < n ? p.y + tokens[tok] * p.y_stride + row : nullptr,
-                                                   tok < n ? p.rows - row : 0);
-            }
+        for (int e = 0; e < 2; ++e) {
+            const int tok = 8 * j + t4 / 2 + e;
+            mine[j][e] = tok < n;
+            y[j][e] = p.y + tokens[tok < n ? tok : 0] * p.y_stride + row_first + 4 * g;
         }
-        float acc[2][NT][4] = {};
-        for (int u = 0; u < units; ++u) {
-            const int r = 16 * u + t4;
-            LoraRaw<W> wt[4];
+    }
+    const LoraRaw<W> last_mask = lora_mask<W>(rank - 16 * (units - 1) - t4);
+    const auto rows = [&](int have, auto whole) {  // kSpan rows, of which the lane has `have` from its first on (whole: all)
+        constexpr bool kWhole = decltype(whole)::value;
+        uint4 old[RG][NT][2];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                wt[i] = lora_load4<W, VEC>(b + static_cast<int64_t>(row + i) * p.max_rank + r,
-                                           row + i < p.rows ? rank - r : 0);
+        for (int q = 0; q < RG; ++q) {
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-                const int at = (8 * j + g) * stride + r;
-                const uint4 h4 = *reinterpret_cast<const uint4 *>(hs + at), l4 = *reinterpret_cast<const uint4 *>(ls + at);
-                const uint32_t hi[4] = {h4.x, h4.y, h4.z, h4.w}, lo[4] = {l4.x, l4.y, l4.z, l4.w};
-                lora_unit<sizeof(W) == 4>(acc[0][j], lora_f32<W>(wt[0]), lora_f32<W>(wt[1]), hi, lo);
-                lora_unit<sizeof(W) == 4>(acc[1][j], lora_f32<W>(wt[2]), lora_f32<W>(wt[3]), hi, lo);
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    old[q][j][e] = lora_load4<float, VEC>(y[j][e] + kLoraRows * q, kWhole ? 4 : have - kLoraRows * q);
             }
         }
+        float acc[RG][2][NT][4] = {};
+        for (int u = 0; u < units; u += KU) {
+            LoraRaw<W> wt[KU][RG][4];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
+            for (int k = 0; k < KU; ++k) {
+                const int at = 16 * min(u + k, units - 1);
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int tok = 8 * j + t4 / 2 + e;
-                if (tok >= n || row >= p.rows) continue;
-                const float4 o = lora_f32<float>(old[j][e]);
-                const float v[4] = {fmaf(scale, acc[0][j][e], o.x), fmaf(scale, acc[0][j][2 + e], o.y),
-                                    fmaf(scale, acc[1][j][e], o.z), fmaf(scale, acc[1][j][2 + e], o.w)};
-                float *y = p.y + tokens[tok] * p.y_stride + row;
-                if (VEC) {
-                    *reinterpret_cast<float4 *>(y) = make_float4(v[0], v[1], v[2], v[3]);
-                } else {
+                for (int q = 0; q < RG; ++q) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (row + i < p.rows) y[i] = v[i];
+                    for (int i = 0; i < 4; ++i) {
+                        const int left = kWhole || have > kLoraRows * q + i ? rank - at - t4 : 0;
+                        wt[k][q][i] = lora_load4<W, VEC>(wr + (kLoraRows * q + i) * p.max_rank + at,
+                                                         VEC ? (kWhole || left ? 4 : 0) : left);
+                    }
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < KU; ++k) {
+                if (u + k >= units) break;
+                if (u + k == units - 1) {
+#pragma unroll
+                    for (int q = 0; q < RG; ++q) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) lora_keep(wt[k][q][i], last_mask);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    const int at = (8 * j + g) * stride + 16 * (u + k) + t4;
+                    const uint4 h4 = *reinterpret_cast<const uint4 *>(hs + at);
+                    const uint4 l4 = *reinterpret_cast<const uint4 *>(ls + at);
+                    const uint32_t hi[4] = {h4.x, h4.y, h4.z, h4.w}, lo[4] = {l4.x, l4.y, l4.z, l4.w};
+#pragma unroll
+                    for (int q = 0; q < RG; ++q) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+                            lora_unit<sizeof(W) == 4>(acc[q][i][j], lora_f32<W>(wt[k][q][2 * i]),
+                                                      lora_f32<W>(wt[k][q][2 * i + 1]), hi, lo);
+                    }
                 }
             }
         }
+#pragma unroll
+        for (int q = 0; q < RG; ++q) {
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float4 o = lora_f32<float>(old[q][j][e]);
+                    const float v[4] = {fmaf(scale, acc[q][0][j][e], o.x), fmaf(scale, acc[q][0][j][2 + e], o.y),
+                                        fmaf(scale, acc[q][1][j][e], o.z), fmaf(scale, acc[q][1][j][2 + e], o.w)};
+                    float *to = y[j][e] + kLoraRows * q;
+                    if (VEC) {
+                        if (mine[j][e] && (kWhole || have > kLoraRows * q))
+                            *reinterpret_cast<float4 *>(to) = make_float4(v[0], v[1], v[2], v[3]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (mine[j][e] && (kWhole || have > kLoraRows * q + i)) to[i] = v[i];
+                    }
+                }
+            }
+        }
+    };
+    for (int row = row_first; row < row_end; row += kLoraWarps * kSpan) {
+        if (row + kSpan <= p.rows) rows(kSpan, std::true_type{});
+        else rows(p.rows - row - 4 * g, std::false_type{});
+        wr += static_cast<int64_t>(kLoraWarps * kSpan) * p.max_rank;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) y[j][0] += kLoraWarps * kSpan, y[j][1] += kLoraWarps * kSpan;
     }
 }
 
@@ -422,17 +531,9 @@ LoraLayout lora_layout(int64_t tokens, int64_t adapters, int64_t max_rank) {
     return l;
 }
 
-template <class W, int MT, int MW, int NT>
-int32_t lora_shrink(const LoraArgs &p, dim3 grid, bool vec, cudaStream_t stream) {
-    if (vec) lora_shrink_kernel<W, MT, MW, NT, true><<<grid, kLoraThreads, 0, stream>>>(p);
-    else lora_shrink_kernel<W, MT, MW, NT, false><<<grid, kLoraThreads, 0, stream>>>(p);
-    return launch_status("lora_shrink_kernel");
-}
-
-template <class W, int NT, bool VEC>
-int32_t lora_expand(const LoraArgs &p, dim3 grid, cudaStream_t stream) {
-    const size_t smem = sizeof(float) * 2 * 8 * NT * (16 * lora_ceil(p.max_rank, 16) + 4);
-    if (const int32_t rc = allow_dynamic_smem(lora_expand_kernel<W, NT, VEC>, smem, "lora_expand smem")) return rc;
+// Launches `kernel`, which waits itself for the kernel before it where it needs it.
+template <class K>
+int32_t lora_start(K *kernel, dim3 grid, size_t smem, const LoraArgs &p, bool early, cudaStream_t stream, const char *name) {
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -442,13 +543,20 @@ int32_t lora_expand(const LoraArgs &p, dim3 grid, cudaStream_t stream) {
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    GLMVX_CUDA(cudaLaunchKernelEx(&cfg, lora_expand_kernel<W, NT, VEC>, p));
-    return launch_status("lora_expand_kernel");
+    cfg.numAttrs = early ? 1 : 0;
+    GLMVX_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
+    return launch_status(name);
+}
+
+template <class W, int MT, int MW, int NT>
+int32_t lora_shrink(const LoraArgs &p, dim3 grid, bool vec, cudaStream_t stream) {
+    return lora_start(vec ? lora_shrink_kernel<W, MT, MW, NT, true> : lora_shrink_kernel<W, MT, MW, NT, false>, grid, 0, p,
+                      p.tiles, stream, "lora_shrink_kernel");
 }
 
 template <class W, int NT>
 int32_t lora_launch(LoraArgs &p, bool vec_a, bool vec_b, cudaStream_t stream) {
+    constexpr int kRG = NT == 1 ? 2 : 1;
     const int sms = sm_count();
     // CTAs along the tokens: every token may lead a tile, or the plan's most.
     const int tiles = p.tiles ? static_cast<int>(std::min<int64_t>(p.tokens, p.tokens / (8 * NT) + int64_t{p.adapters}))
@@ -469,10 +577,15 @@ int32_t lora_launch(LoraArgs &p, bool vec_a, bool vec_b, cudaStream_t stream) {
     else if (ranks == 32) rc = lora_shrink<W, 2, 1, NT>(p, grid, vec_a, stream);
     else rc = lora_shrink<W, 2, 2, NT>(p, grid, vec_a, stream);
     if (rc) return rc;
-    const int steps = lora_ceil(p.rows, kLoraWarps * kLoraRows);
-    p.row_steps = std::max(1, static_cast<int>(int64_t{steps} * full / (8 * sms)));
+    // Rows in as many parts as give eight CTAs an SM if every CTA has a tile.
+    const int steps = lora_ceil(p.rows, kLoraWarps * kLoraRows * kRG);
+    p.row_steps = std::max(1, static_cast<int>(int64_t{steps} * tiles / (8 * sms)));
     const dim3 out(tiles, lora_ceil(steps, p.row_steps));
-    return vec_b ? lora_expand<W, NT, true>(p, out, stream) : lora_expand<W, NT, false>(p, out, stream);
+    const size_t smem = sizeof(float) * 2 * 8 * NT * 16 * (lora_ceil(p.max_rank, 16) | 1);
+    const auto expand = p.max_rank <= 16 ? (vec_b ? lora_expand_kernel<W, NT, kRG, 1, true> : lora_expand_kernel<W, NT, kRG, 1, false>)
+                                         : (vec_b ? lora_expand_kernel<W, NT, kRG, 2, true> : lora_expand_kernel<W, NT, kRG, 2, false>);
+    if (const int32_t e = allow_dynamic_smem(expand, smem, "lora_expand smem")) return e;
+    return lora_start(expand, out, smem, p, true, stream, "lora_expand_kernel");
 }
 
 }  // namespace
@@ -529,8 +642,8 @@ GLMVX_EXPORT int32_t glmvx_lora_add(float *y, int64_t y_stride, const float *x, 
     const bool vec_b = !(max_rank & 3) && !(rows & 3) && !(bits(b) & four) && !(bits(y) & 15) &&
                        (tokens == 1 || !(y_stride & 3));
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const bool wide = tokens > 64;
-    if (kind == 0) return wide ? lora_launch<float, 4>(p, vec_a, vec_b, s) : lora_launch<float, 1>(p, vec_a, vec_b, s);
-    if (kind == 1) return wide ? lora_launch<__half, 4>(p, vec_a, vec_b, s) : lora_launch<__half, 1>(p, vec_a, vec_b, s);
-    return wide ? lora_launch<__nv_bfloat16, 4>(p, vec_a, vec_b, s) : lora_launch<__nv_bfloat16, 1>(p, vec_a, vec_b, s);
+    const bool wide = tokens > kLoraScan;
+    if (kind == 0) return wide ? lora_launch<float, 2>(p, vec_a, vec_b, s) : lora_launch<float, 1>(p, vec_a, vec_b, s);
+    if (kind == 1) return wide ? lora_launch<__half, 2>(p, vec_a, vec_b, s) : lora_launch<__half, 1>(p, vec_a, vec_b, s);
+    return wide ? lora_launch<__nv_bfloat16, 2>(p, vec_a, vec_b, s) : lora_launch<__nv_bfloat16, 1>(p, vec_a, vec_b, s);
 }
