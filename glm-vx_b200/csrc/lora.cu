@@ -269,14 +269,14 @@ __global__ void __launch_bounds__(kLoraPlanThreads) lora_plan_kernel(LoraArgs p,
 
 // h[split][token][r] = A[r][the split's columns] . x[token][the split's columns]
 // for a tile of 8 NT tokens and 16 MT MW ranks (blockIdx.z: which).  MW warps
-// share a unit of 16 columns, 16 MT ranks each, and take every 8 / MW-th unit, two
-// at a time, the next two on their way meanwhile; the warps' sums are joined in
+// share a unit of 16 columns, 16 MT ranks each, and take every 8 / MW-th pair of
+// neighbouring units, the next pair on its way meanwhile; the warps' sums are joined in
 // order.  Lanes without a token or a rank of their own read the first one's:
 // what they make is a column or a row of the tile that nobody keeps.
 template <class W, int MT, int MW, int NT, bool VEC>
 __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(LoraArgs p) {
     constexpr int kUnits = 2, kKWarps = kLoraWarps / MW, kRanks = 16 * MT * MW, kStride = 8 * NT + 1;
-    constexpr int kStep = 16 * kKWarps;  // columns from a warp's unit to its next
+    constexpr int kBatch = 16 * kUnits * kKWarps;  // columns from a warp's units to its next
     __shared__ int tokens[8 * NT], n;
     __shared__ float parts[kKWarps][kRanks * kStride];
     grid_dependency_wait();  // the plan comes from the kernel before
@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(LoraArgs p
     if (r0 >= rank) return;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = 4 * (lane & 3);
     const int kw = warp / MW, rw = r0 + 16 * MT * (warp % MW) + g;  // the lane's first rank
-    const int split = blockIdx.y, u0 = split * p.units + kw, u1 = min((split + 1) * p.units, (p.cols + 15) / 16);
+    const int split = blockIdx.y, u0 = split * p.units + kUnits * kw, u1 = min((split + 1) * p.units, (p.cols + 15) / 16);
     const W *w[2 * MT];
     const float *x[NT];
 #pragma unroll
@@ -306,14 +306,14 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(LoraArgs p
 #pragma unroll
         for (int k = 0; k < kUnits; ++k) {
 #pragma unroll
-            for (int j = 0; j < NT; ++j) t.x[k][j] = lora_load4<float, VEC>(x[j] + k * kStep, left - k * kStep);
+            for (int j = 0; j < NT; ++j) t.x[k][j] = lora_load4<float, VEC>(x[j] + 16 * k, left - 16 * k);
 #pragma unroll
-            for (int i = 0; i < 2 * MT; ++i) t.w[k][i] = lora_load4<W, VEC>(w[i] + k * kStep, left - k * kStep);
+            for (int i = 0; i < 2 * MT; ++i) t.w[k][i] = lora_load4<W, VEC>(w[i] + 16 * k, left - 16 * k);
         }
 #pragma unroll
-        for (int j = 0; j < NT; ++j) x[j] += kUnits * kStep;
+        for (int j = 0; j < NT; ++j) x[j] += kBatch;
 #pragma unroll
-        for (int i = 0; i < 2 * MT; ++i) w[i] += kUnits * kStep;
+        for (int i = 0; i < 2 * MT; ++i) w[i] += kBatch;
     };
     const auto multiply = [&](const Batch &t) {
 #pragma unroll
@@ -331,7 +331,6 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(LoraArgs p
     };
     Batch even, odd;
     int left = min(p.cols, 16 * u1) - (16 * u0 + t4);
-    constexpr int kBatch = kUnits * kStep;
     // left + t4 is what the warp's first lane has left: the same in all lanes
     load(even, left);
     while (left + t4 > 0) {
@@ -369,7 +368,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(LoraArgs p
 // g of half i of two m16 tiles, so that a lane ends up with four neighbouring
 // rows of two tokens: one float4 of y each.  KU units of 16 ranks are read at once.
 template <class W, int NT, int RG, int KU, bool VEC>
-__global__ void __launch_bounds__(kLoraThreads, sizeof(W) == 4 ? 2 : 3) lora_expand_kernel(LoraArgs p) {
+__global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(LoraArgs p) {
     extern __shared__ __align__(16) float hs[];  // [2][8 NT][stride]: hi, lo
     __shared__ int tokens[8 * NT], n;
     const int a = lora_tile<8 * NT>(p, tokens, n, false);
@@ -418,18 +417,21 @@ __global__ void __launch_bounds__(kLoraThreads, sizeof(W) == 4 ? 2 : 3) lora_exp
         }
     }
     const LoraRaw<W> last_mask = lora_mask<W>(rank - 16 * (units - 1) - t4);
-    const auto rows = [&](int have, auto whole) {  // kSpan rows, of which the lane has `have` from its first on (whole: all)
-        constexpr bool kWhole = decltype(whole)::value;
-        uint4 old[RG][NT][2];
+    // y's rows of a step, a step ahead.
+    uint4 old[RG][NT][2], next[RG][NT][2];
+    const auto fetch = [&](uint4(&to)[RG][NT][2], int64_t on, int have) {
 #pragma unroll
         for (int q = 0; q < RG; ++q) {
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
-                    old[q][j][e] = lora_load4<float, VEC>(y[j][e] + kLoraRows * q, kWhole ? 4 : have - kLoraRows * q);
+                    to[q][j][e] = lora_load4<float, VEC>(y[j][e] + on + kLoraRows * q, have - kLoraRows * q);
             }
         }
+    };
+    const auto rows = [&](int have, auto whole) {  // kSpan rows, of which the lane has `have` from its first on (whole: all)
+        constexpr bool kWhole = decltype(whole)::value;
         float acc[RG][2][NT][4] = {};
         for (int u = 0; u < units; u += KU) {
             LoraRaw<W> wt[KU][RG][4];
@@ -494,12 +496,22 @@ __global__ void __launch_bounds__(kLoraThreads, sizeof(W) == 4 ? 2 : 3) lora_exp
             }
         }
     };
-    for (int row = row_first; row < row_end; row += kLoraWarps * kSpan) {
+    constexpr int kNext = kLoraWarps * kSpan;
+    fetch(old, 0, p.rows - row_first - 4 * g);
+    for (int row = row_first; row < row_end; row += kNext) {
+        if (row + kNext < row_end) fetch(next, kNext, p.rows - row - kNext - 4 * g);
         if (row + kSpan <= p.rows) rows(kSpan, std::true_type{});
         else rows(p.rows - row - 4 * g, std::false_type{});
-        wr += static_cast<int64_t>(kLoraWarps * kSpan) * p.max_rank;
+        wr += static_cast<int64_t>(kNext) * p.max_rank;
 #pragma unroll
-        for (int j = 0; j < NT; ++j) y[j][0] += kLoraWarps * kSpan, y[j][1] += kLoraWarps * kSpan;
+        for (int j = 0; j < NT; ++j) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                y[j][e] += kNext;
+#pragma unroll
+                for (int q = 0; q < RG; ++q) old[q][j][e] = next[q][j][e];
+            }
+        }
     }
 }
 
