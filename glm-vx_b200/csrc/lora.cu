@@ -52,7 +52,7 @@ struct LoraArgs {
     LoraTile *tiles;  // the plan (NULL: CTAs scan the ids)
     int *order, *counts, *places, *ntiles;
     int64_t y_stride, x_stride;
-    int tokens, rows, cols, adapters, max_rank, splits, units, row_steps;
+    int tokens, rows, cols, adapters, max_rank, splits, units;
     int *err;
 };
 
@@ -161,53 +161,75 @@ __device__ __forceinline__ void lora_unit(float (&c)[4], const float4 &top, cons
     for (int s = 0; s < 4; s += 2) lora_mma(c, th[s], lh[s], th[s + 1], lh[s + 1], hi[s], hi[s + 1]);
 }
 
-// The tile of this CTA (blockIdx.x): its adapter (-1: no tile), its tokens and their number.  With a
-// plan it is the plan's.  Without, CTA t leads a tile if token t is the first, or
-// TILE-th, 2 TILE-th ..., of its adapter's tokens; the tile is t and the next ones.
+// The tiles of a call as a CTA knows them: the plan's, or (few tokens) a table that
+// each CTA makes for itself: a token leads a tile if it is the first, or TILE-th,
+// 2 TILE-th ..., of its adapter's tokens; the tile is it and the next ones.
 template <int TILE>
-__device__ __forceinline__ int lora_tile(const LoraArgs &p, int (&tokens)[TILE], int &n, bool report) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, t = blockIdx.x;
+struct LoraTiles {
+    int count;
+    int tokens[TILE], adapter, n;  // of the tile last opened
+    int ids[kLoraScan], leads[kLoraScan / 32];
+    int tile_adapter[kLoraScan], tile_n[kLoraScan], tile_tokens[kLoraScan][TILE];
+};
+
+template <int TILE>
+__device__ __forceinline__ void lora_tiles(LoraTiles<TILE> &s, const LoraArgs &p, bool report) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (p.tiles) {
-        if (t >= *p.ntiles) return -1;
-        const LoraTile tile = p.tiles[t];
-        for (int i = tid; i < tile.n; i += kLoraThreads) tokens[i] = p.order[tile.start + i];
-        if (tid == 0) n = tile.n;
+        if (tid == 0) s.count = *p.ntiles;
         __syncthreads();
-        return tile.adapter;
+        return;
     }
-    __shared__ uint32_t match[kLoraScan / 32];
-    const int a = p.ids[t];
-    if (a >= p.adapters && report && tid == 0) report_device_error(p.err, kDevErrBadIndex);
-    if (a < 0 || a >= p.adapters) return -1;
-    const int words = (p.tokens + 31) / 32;
-    for (int w = warp; w < words; w += kLoraWarps) {
-        const int j = 32 * w + lane;
-        const uint32_t m = __ballot_sync(0xffffffffu, j < p.tokens && p.ids[j] == a);
-        if (lane == 0) match[w] = m;
-    }
-    __syncthreads();
-    if (warp == 0) {
-        const uint32_t m = lane < words ? match[lane] : 0u;
-        const int mine = __popc(m);
-        int before = mine;  // matches in the words before this lane's
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int up = __shfl_up_sync(0xffffffffu, before, o);
-            if (lane >= o) before += up;
+    int a = -1;
+    if (tid < kLoraScan) {
+        a = tid < p.tokens ? p.ids[tid] : -1;
+        if (a >= p.adapters) {
+            if (report) report_device_error(p.err, kDevErrBadIndex);
+            a = -1;
         }
-        const int all = __shfl_sync(0xffffffffu, before, 31);
-        before -= mine;
-        const int lead = __shfl_sync(0xffffffffu, before + __popc(m & ((1u << (t & 31)) - 1)), t >> 5);
-        const int here = lead % TILE ? 0 : min(TILE, all - lead);
-        if (here)
-            for (uint32_t left = m, r = before; left; left &= left - 1, ++r) {
-                const int at = static_cast<int>(r) - lead;
-                if (at >= 0 && at < here) tokens[at] = 32 * lane + __ffs(left) - 1;
-            }
-        if (lane == 0) n = here;
+        s.ids[tid] = a;
     }
     __syncthreads();
-    return n ? a : -1;
+    uint64_t same = 0;  // the tokens of this one's adapter
+    if (tid < kLoraScan) {
+#pragma unroll 8
+        for (int j = 0; j < kLoraScan; ++j) same |= static_cast<uint64_t>(s.ids[j] == a) << j;
+        const bool leads = a >= 0 && __popcll(same & ((1ull << tid) - 1)) % TILE == 0;
+        const uint32_t m = __ballot_sync(0xffffffffu, leads);
+        if (lane == 0) s.leads[warp] = m;
+        if (!leads) same = 0;
+    }
+    __syncthreads();
+    if (tid < kLoraScan && same) {
+        int k = __popc(s.leads[warp] & ((1u << lane) - 1));
+        for (int w = 0; w < warp; ++w) k += __popc(s.leads[w]);
+        int n = 0;
+        for (uint64_t left = same >> tid << tid; left && n < TILE; left &= left - 1) s.tile_tokens[k][n++] = __ffsll(left) - 1;
+        s.tile_adapter[k] = a;
+        s.tile_n[k] = n;
+    }
+    if (tid == 0) {
+        int all = 0;
+        for (int w = 0; w < kLoraScan / 32; ++w) all += __popc(s.leads[w]);
+        s.count = all;
+    }
+    __syncthreads();
+}
+
+// Opens tile k: its adapter, its tokens (of those it lacks, its first).
+template <int TILE>
+__device__ __forceinline__ void lora_open(LoraTiles<TILE> &s, const LoraArgs &p, int k) {
+    __syncthreads();  // the tile before is done with
+    const int tid = threadIdx.x;
+    if (p.tiles) {
+        const LoraTile tile = p.tiles[k];
+        if (tid < TILE) s.tokens[tid] = p.order[tile.start + (tid < tile.n ? tid : 0)];
+        if (tid == 0) s.adapter = tile.adapter, s.n = tile.n;
+    } else {
+        if (tid < TILE) s.tokens[tid] = s.tile_tokens[k][tid < s.tile_n[k] ? tid : 0];
+        if (tid == 0) s.adapter = s.tile_adapter[k], s.n = s.tile_n[k];
+    }
+    __syncthreads();
 }
 
 // Tiles of up to `tile` tokens of one adapter: one CTA counts the adapters'
@@ -268,7 +290,7 @@ __global__ void __launch_bounds__(kLoraPlanThreads) lora_plan_kernel(LoraArgs p,
 }
 
 // h[split][token][r] = A[r][the split's columns] . x[token][the split's columns]
-// for a tile of 8 NT tokens and 16 MT MW ranks (blockIdx.z: which).  MW warps
+// for a tile of 8 NT tokens and 16 MT MW ranks, item after item.  MW warps
 // share a unit of 16 columns, 16 MT ranks each, and take every 8 / MW-th pair of
 // neighbouring units, the next pair on its way meanwhile; the warps' sums are joined in
 // order.  Lanes without a token or a rank of their own read the first one's:
@@ -277,17 +299,20 @@ template <class W, int MT, int MW, int NT, bool VEC>
 __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(LoraArgs p) {
     constexpr int kUnits = 2, kKWarps = kLoraWarps / MW, kRanks = 16 * MT * MW, kStride = 8 * NT + 1;
     constexpr int kBatch = 16 * kUnits * kKWarps;  // columns from a warp's units to its next
-    __shared__ int tokens[8 * NT], n;
+    __shared__ LoraTiles<8 * NT> tiles;
     __shared__ float parts[kKWarps][kRanks * kStride];
     grid_dependency_wait();  // the plan comes from the kernel before
     allow_dependent_launch();
-    const int a = lora_tile<8 * NT>(p, tokens, n, blockIdx.y == 0 && blockIdx.z == 0);
-    if (a < 0) return;
-    const int rank = lora_rank(p, a), r0 = blockIdx.z * kRanks;
-    if (r0 >= rank) return;
+    lora_tiles(tiles, p, blockIdx.x == 0);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = 4 * (lane & 3);
+    const int chunks = (p.max_rank + kRanks - 1) / kRanks, per_tile = p.splits * chunks;
+    for (int64_t item = blockIdx.x; item < static_cast<int64_t>(tiles.count) * per_tile; item += gridDim.x) {
+    lora_open(tiles, p, static_cast<int>(item / per_tile));
+    const int part = static_cast<int>(item % per_tile), split = part / chunks, r0 = part % chunks * kRanks;
+    const int a = tiles.adapter, n = tiles.n, rank = lora_rank(p, a);
+    if (r0 >= rank) continue;
     const int kw = warp / MW, rw = r0 + 16 * MT * (warp % MW) + g;  // the lane's first rank
-    const int split = blockIdx.y, u0 = split * p.units + kUnits * kw, u1 = min((split + 1) * p.units, (p.cols + 15) / 16);
+    const int u0 = split * p.units + kUnits * kw, u1 = min((split + 1) * p.units, (p.cols + 15) / 16);
     const W *w[2 * MT];
     const float *x[NT];
 #pragma unroll
@@ -296,7 +321,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(LoraArgs p
         w[i] = static_cast<const W *>(p.a) + (static_cast<int64_t>(a) * p.max_rank + r) * p.cols + 16 * u0 + t4;
     }
 #pragma unroll
-    for (int j = 0; j < NT; ++j) x[j] = p.x + tokens[8 * j + g < n ? 8 * j + g : 0] * p.x_stride + 16 * u0 + t4;
+    for (int j = 0; j < NT; ++j) x[j] = p.x + tiles.tokens[8 * j + g] * p.x_stride + 16 * u0 + t4;
     float acc[MT][NT][4] = {};
     struct Batch {
         LoraRaw<W> w[kUnits][2 * MT];
@@ -359,160 +384,179 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(LoraArgs p
         float sum = 0.0f;
 #pragma unroll
         for (int v = 0; v < kKWarps; ++v) sum += parts[v][r * kStride + tok];
-        p.h[(static_cast<int64_t>(split) * p.tokens + tokens[tok]) * p.max_rank + r0 + r] = sum;
+        p.h[(static_cast<int64_t>(split) * p.tokens + tiles.tokens[tok]) * p.max_rank + r0 + r] = sum;
+    }
     }
 }
 
-// y[token][row] += s * B[row] . h[token] for a tile of 8 NT tokens; blockIdx.y takes
-// row_steps groups of 32 RG rows per warp.  Row 4 g + i of 32 stands at place
-// g of half i of two m16 tiles, so that a lane ends up with four neighbouring
-// rows of two tokens: one float4 of y each.  KU units of 16 ranks are read at once.
+// y[token][row] += s * B[row] . h[token] for tiles of 8 NT tokens.  A CTA's share is
+// a run of the steps of all tiles (a step: 32 RG rows a warp).  Row 4 g + i of
+// 32 stands at place g of half i of two m16 tiles, so that a lane ends up with
+// four neighbouring rows of two tokens: one float4 of y each.  y and the weights
+// (KU units of 16 ranks at once) are read one step, or KU units, ahead.  With VEC
+// lanes whose rows are behind the last read the last ones and write nothing.
 template <class W, int NT, int RG, int KU, bool VEC>
 __global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(LoraArgs p) {
-    extern __shared__ __align__(16) float hs[];  // [2][8 NT][stride]: hi, lo
-    __shared__ int tokens[8 * NT], n;
-    const int a = lora_tile<8 * NT>(p, tokens, n, false);
-    if (a < 0) return;
-    const int rank = lora_rank(p, a), units = (rank + 15) / 16;
-    const int stride = 16 * (units | 1);  // 16 mod 32 banks: the quarters of a warp's 16-byte reads do not meet
-    if (rank == 0) return;
-    const float scale = p.scales[a];
+    extern __shared__ __align__(16) float hs[];  // [2][8 NT][pitch]: hi, lo
+    __shared__ LoraTiles<8 * NT> tiles;
+    constexpr int kSpan = kLoraRows * RG, kNext = kLoraWarps * kSpan;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = 4 * (lane & 3);
-    float *ls = hs + 8 * NT * stride;
-    grid_dependency_wait();  // h comes from the kernel before
-    for (int i = tid; i < 8 * NT * 16 * units; i += kLoraThreads) {
-        const int tok = i / (16 * units), r = i - tok * 16 * units;
-        float sum = 0.0f;
-        if (tok < n && r < rank) {
-            const float *h = p.h + static_cast<int64_t>(tokens[tok]) * p.max_rank + r;
-            const int64_t next = static_cast<int64_t>(p.tokens) * p.max_rank;
-            for (int s = 0; s < p.splits; s += 8) {  // in order, eight in flight
-                float part[8];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) part[k] = s + k < p.splits ? h[(s + k) * next] : 0.0f;
-#pragma unroll
-                for (int k = 0; k < 8; ++k) sum += part[k];
-            }
-        }
-        const uint32_t hi = lora_tf32(sum);
-        hs[tok * stride + r] = __uint_as_float(hi);
-        ls[tok * stride + r] = __uint_as_float(lora_tf32(sum - __uint_as_float(hi)));
-    }
-    __syncthreads();
-    // The lane's rows of B, and its tokens' rows of y from the warp's first row on; a lane without a
-    // token has the first one's, which it reads and does not write.
-    constexpr int kSpan = kLoraRows * RG;
-    const int row_first = (blockIdx.y * p.row_steps * kLoraWarps + warp) * kSpan;
-    const int row_end = min(p.rows, row_first + (p.row_steps - 1) * kLoraWarps * kSpan + kSpan);
-    const W *wr = static_cast<const W *>(p.b) + (static_cast<int64_t>(a) * p.rows + row_first + 4 * g) * p.max_rank + t4;
-    float *y[NT][2];
-    bool mine[NT][2];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int tok = 8 * j + t4 / 2 + e;
-            mine[j][e] = tok < n;
-            y[j][e] = p.y + tokens[tok < n ? tok : 0] * p.y_stride + row_first + 4 * g;
-        }
-    }
-    const LoraRaw<W> last_mask = lora_mask<W>(rank - 16 * (units - 1) - t4);
-    // y's rows of a step, a step ahead.
-    uint4 old[RG][NT][2], next[RG][NT][2];
-    const auto fetch = [&](uint4(&to)[RG][NT][2], int64_t on, int have) {
-#pragma unroll
-        for (int q = 0; q < RG; ++q) {
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-#pragma unroll
-                for (int e = 0; e < 2; ++e)
-                    to[q][j][e] = lora_load4<float, VEC>(y[j][e] + on + kLoraRows * q, have - kLoraRows * q);
-            }
-        }
-    };
-    const auto rows = [&](int have, auto whole) {  // kSpan rows, of which the lane has `have` from its first on (whole: all)
-        constexpr bool kWhole = decltype(whole)::value;
-        float acc[RG][2][NT][4] = {};
-        for (int u = 0; u < units; u += KU) {
-            LoraRaw<W> wt[KU][RG][4];
-#pragma unroll
-            for (int k = 0; k < KU; ++k) {
-                const int at = 16 * min(u + k, units - 1);
-#pragma unroll
-                for (int q = 0; q < RG; ++q) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int left = kWhole || have > kLoraRows * q + i ? rank - at - t4 : 0;
-                        wt[k][q][i] = lora_load4<W, VEC>(wr + (kLoraRows * q + i) * p.max_rank + at,
-                                                         VEC ? (kWhole || left ? 4 : 0) : left);
-                    }
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < KU; ++k) {
-                if (u + k >= units) break;
-                if (u + k == units - 1) {
-#pragma unroll
-                    for (int q = 0; q < RG; ++q) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) lora_keep(wt[k][q][i], last_mask);
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    const int at = (8 * j + g) * stride + 16 * (u + k) + t4;
-                    const uint4 h4 = *reinterpret_cast<const uint4 *>(hs + at);
-                    const uint4 l4 = *reinterpret_cast<const uint4 *>(ls + at);
-                    const uint32_t hi[4] = {h4.x, h4.y, h4.z, h4.w}, lo[4] = {l4.x, l4.y, l4.z, l4.w};
-#pragma unroll
-                    for (int q = 0; q < RG; ++q) {
-#pragma unroll
-                        for (int i = 0; i < 2; ++i)
-                            lora_unit<sizeof(W) == 4>(acc[q][i][j], lora_f32<W>(wt[k][q][2 * i]),
-                                                      lora_f32<W>(wt[k][q][2 * i + 1]), hi, lo);
-                    }
-                }
-            }
-        }
-#pragma unroll
-        for (int q = 0; q < RG; ++q) {
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float4 o = lora_f32<float>(old[q][j][e]);
-                    const float v[4] = {fmaf(scale, acc[q][0][j][e], o.x), fmaf(scale, acc[q][0][j][2 + e], o.y),
-                                        fmaf(scale, acc[q][1][j][e], o.z), fmaf(scale, acc[q][1][j][2 + e], o.w)};
-                    float *to = y[j][e] + kLoraRows * q;
-                    if (VEC) {
-                        if (mine[j][e] && (kWhole || have > kLoraRows * q))
-                            *reinterpret_cast<float4 *>(to) = make_float4(v[0], v[1], v[2], v[3]);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (mine[j][e] && (kWhole || have > kLoraRows * q + i)) to[i] = v[i];
-                    }
-                }
-            }
-        }
-    };
-    constexpr int kNext = kLoraWarps * kSpan;
-    fetch(old, 0, p.rows - row_first - 4 * g);
-    for (int row = row_first; row < row_end; row += kNext) {
-        if (row + kNext < row_end) fetch(next, kNext, p.rows - row - kNext - 4 * g);
-        if (row + kSpan <= p.rows) rows(kSpan, std::true_type{});
-        else rows(p.rows - row - 4 * g, std::false_type{});
-        wr += static_cast<int64_t>(kNext) * p.max_rank;
+    lora_tiles(tiles, p, false);
+    bool waited = false;
+    const int per_tile = (p.rows + kNext - 1) / kNext;
+    const int64_t all = static_cast<int64_t>(tiles.count) * per_tile;
+    int64_t at = all * blockIdx.x / gridDim.x;
+    const int64_t end = all * (blockIdx.x + 1) / gridDim.x;
+    while (at < end) {
+        lora_open(tiles, p, static_cast<int>(at / per_tile));
+        const int first = static_cast<int>(at % per_tile);
+        const int steps = static_cast<int>(min(end - at, static_cast<int64_t>(per_tile - first)));
+        at += steps;
+        const int a = tiles.adapter, n = tiles.n, rank = lora_rank(p, a), units = (rank + 15) / 16;
+        if (rank == 0) continue;
+        const int pitch = 16 * (units | 1);  // 16 mod 32 banks: the quarters of a warp's 16-byte reads do not meet
+        const float scale = p.scales[a];
+        float *ls = hs + 8 * NT * pitch;
+        const W *b = static_cast<const W *>(p.b) + static_cast<int64_t>(a) * p.rows * p.max_rank + t4;
+        float *y[NT][2];  // the lane's tokens' rows
+        bool mine[NT][2];
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                y[j][e] += kNext;
-#pragma unroll
-                for (int q = 0; q < RG; ++q) old[q][j][e] = next[q][j][e];
+                const int tok = 8 * j + t4 / 2 + e;
+                mine[j][e] = tok < n;
+                y[j][e] = p.y + tiles.tokens[tok] * p.y_stride;
             }
         }
+        struct Rows {
+            float v[RG][NT][2][4];
+        };
+        struct Weights {
+            LoraRaw<W> w[KU][RG][4];
+        };
+        const auto load_y = [&](Rows &to, int row) {
+#pragma unroll
+            for (int q = 0; q < RG; ++q) {
+                const int r = row + kLoraRows * q;
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        if (VEC) {
+                            *reinterpret_cast<float4 *>(to.v[q][j][e]) =
+                                *reinterpret_cast<const float4 *>(y[j][e] + min(r, p.rows - 4));
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) to.v[q][j][e][i] = y[j][e][min(r + i, p.rows - 1)];
+                        }
+                    }
+                }
+            }
+        };
+        const auto load_w = [&](Weights &to, int row, int u) {
+#pragma unroll
+            for (int q = 0; q < RG; ++q) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = min(row + kLoraRows * q + i, VEC ? p.rows - 4 + i : p.rows - 1);
+                    const W *from = b + static_cast<int64_t>(r) * p.max_rank;
+#pragma unroll
+                    for (int k = 0; k < KU; ++k) {
+                        const int c = 16 * min(u + k, units - 1);
+                        if (VEC) to.w[k][q][i] = t4 + c < rank ? __ldg(reinterpret_cast<const LoraRaw<W> *>(from + c)) : LoraRaw<W>{};
+                        else to.w[k][q][i] = lora_load4<W, false>(from + c, rank - c - t4);
+                    }
+                }
+            }
+        };
+        int row = (first * kLoraWarps + warp) * kSpan + 4 * g;
+        Rows old, next;
+        Weights wt, ahead;
+        load_y(old, row);
+        load_w(wt, row, 0);
+        // h, its parts joined in order, as hi + lo; zero behind the rank
+        if (!waited) grid_dependency_wait();  // h comes from the kernel before
+        waited = true;
+        for (int i = tid; i < 8 * NT * 16 * units; i += kLoraThreads) {
+            const int tok = i / (16 * units), r = i - tok * 16 * units;
+            float sum = 0.0f;
+            if (tok < n && r < rank) {
+                const float *h = p.h + static_cast<int64_t>(tiles.tokens[tok]) * p.max_rank + r;
+                const int64_t on = static_cast<int64_t>(p.tokens) * p.max_rank;
+                for (int s = 0; s < p.splits; s += 8) {  // eight in flight
+                    float part[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) part[k] = s + k < p.splits ? h[(s + k) * on] : 0.0f;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) sum += part[k];
+                }
+            }
+            const uint32_t hi = lora_tf32(sum);
+            hs[tok * pitch + r] = __uint_as_float(hi);
+            ls[tok * pitch + r] = __uint_as_float(lora_tf32(sum - __uint_as_float(hi)));
+        }
+        __syncthreads();
+        const LoraRaw<W> last_mask = lora_mask<W>(rank - 16 * (units - 1) - t4);
+        for (int step = 0; step < steps; ++step, row += kNext) {
+            if (step + 1 < steps) load_y(next, row + kNext);
+            float acc[RG][2][NT][4] = {};
+            for (int u = 0; u < units; u += KU) {
+                if (u + KU < units) load_w(ahead, row, u + KU);
+                else if (step + 1 < steps) load_w(ahead, row + kNext, 0);
+#pragma unroll
+                for (int k = 0; k < KU; ++k) {
+                    if (u + k >= units) break;
+                    if (u + k == units - 1) {
+#pragma unroll
+                        for (int q = 0; q < RG; ++q) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) lora_keep(wt.w[k][q][i], last_mask);
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        const int from = (8 * j + g) * pitch + 16 * (u + k) + t4;
+                        const uint4 h4 = *reinterpret_cast<const uint4 *>(hs + from);
+                        const uint4 l4 = *reinterpret_cast<const uint4 *>(ls + from);
+                        const uint32_t hi[4] = {h4.x, h4.y, h4.z, h4.w}, lo[4] = {l4.x, l4.y, l4.z, l4.w};
+#pragma unroll
+                        for (int q = 0; q < RG; ++q) {
+#pragma unroll
+                            for (int i = 0; i < 2; ++i)
+                                lora_unit<sizeof(W) == 4>(acc[q][i][j], lora_f32<W>(wt.w[k][q][2 * i]),
+                                                          lora_f32<W>(wt.w[k][q][2 * i + 1]), hi, lo);
+                        }
+                    }
+                }
+                wt = ahead;
+            }
+#pragma unroll
+            for (int q = 0; q < RG; ++q) {
+                const int r = row + kLoraRows * q;
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float *o = old.v[q][j][e];
+                        const float v[4] = {fmaf(scale, acc[q][0][j][e], o[0]), fmaf(scale, acc[q][0][j][2 + e], o[1]),
+                                            fmaf(scale, acc[q][1][j][e], o[2]), fmaf(scale, acc[q][1][j][2 + e], o[3])};
+                        if (VEC) {
+                            if (mine[j][e] && r < p.rows)
+                                *reinterpret_cast<float4 *>(y[j][e] + r) = make_float4(v[0], v[1], v[2], v[3]);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (mine[j][e] && r + i < p.rows) y[j][e][r + i] = v[i];
+                        }
+                    }
+                }
+            }
+            old = next;
+        }
     }
+    // A CTA with nothing to do must not end before the kernel before: what comes next waits for this one only.
+    if (!waited) grid_dependency_wait();
 }
 
 constexpr int lora_ceil(int64_t n, int64_t of) { return static_cast<int>((n + of - 1) / of); }
@@ -566,9 +610,15 @@ int32_t lora_shrink(const LoraArgs &p, dim3 grid, bool vec, cudaStream_t stream)
                       p.tiles, stream, "lora_shrink_kernel");
 }
 
+template <class W, int NT, int RG, int KU>
+int32_t lora_expand(const LoraArgs &p, dim3 grid, size_t smem, bool vec, cudaStream_t stream) {
+    const auto kernel = vec ? lora_expand_kernel<W, NT, RG, KU, true> : lora_expand_kernel<W, NT, RG, KU, false>;
+    if (const int32_t rc = allow_dynamic_smem(kernel, smem, "lora_expand smem")) return rc;
+    return lora_start(kernel, grid, smem, p, true, stream, "lora_expand_kernel");
+}
+
 template <class W, int NT>
 int32_t lora_launch(LoraArgs &p, bool vec_a, bool vec_b, cudaStream_t stream) {
-    constexpr int kRG = NT == 1 ? 2 : 1;
     const int sms = sm_count();
     // CTAs along the tokens: every token may lead a tile, or the plan's most.
     const int tiles = p.tiles ? static_cast<int>(std::min<int64_t>(p.tokens, p.tokens / (8 * NT) + int64_t{p.adapters}))
@@ -577,27 +627,24 @@ int32_t lora_launch(LoraArgs &p, bool vec_a, bool vec_b, cudaStream_t stream) {
         lora_plan_kernel<<<1, kLoraPlanThreads, 0, stream>>>(p, 8 * NT);
         if (const int32_t rc = launch_status("lora_plan_kernel")) return rc;
     }
-    // Columns in as many parts as give four CTAs an SM, none shorter than four units a warp.
+    // Columns in as many parts as give four items an SM were every tile full, none shorter than four units a warp.
     const int full = lora_ceil(p.tokens, 8 * NT), all_units = lora_ceil(p.cols, 16);
     p.splits = std::min({lora_max_splits(p.tokens), lora_ceil(all_units, 4 * kLoraWarps), lora_ceil(4 * sms, full)});
     p.units = lora_ceil(all_units, p.splits);
     p.splits = lora_ceil(all_units, p.units);
     const int ranks = p.max_rank <= 16 ? 16 : p.max_rank <= 32 ? 32 : kLoraRankChunk;
-    const dim3 grid(tiles, p.splits, lora_ceil(p.max_rank, ranks));
+    // Two CTAs an SM share the work, whatever the number of tiles turns out to be; fewer where there is less.
+    const auto ctas = [&](int64_t items) { return dim3(static_cast<unsigned>(std::min<int64_t>(items * tiles, 2 * sms))); };
+    const dim3 grid = ctas(int64_t{p.splits} * lora_ceil(p.max_rank, ranks));
     int32_t rc = kOk;
     if (ranks == 16) rc = lora_shrink<W, 1, 1, NT>(p, grid, vec_a, stream);
     else if (ranks == 32) rc = lora_shrink<W, 2, 1, NT>(p, grid, vec_a, stream);
     else rc = lora_shrink<W, 2, 2, NT>(p, grid, vec_a, stream);
     if (rc) return rc;
-    // Rows in as many parts as give eight CTAs an SM if every CTA has a tile.
-    const int steps = lora_ceil(p.rows, kLoraWarps * kLoraRows * kRG);
-    p.row_steps = std::max(1, static_cast<int>(int64_t{steps} * tiles / (8 * sms)));
-    const dim3 out(tiles, lora_ceil(steps, p.row_steps));
     const size_t smem = sizeof(float) * 2 * 8 * NT * 16 * (lora_ceil(p.max_rank, 16) | 1);
-    const auto expand = p.max_rank <= 16 ? (vec_b ? lora_expand_kernel<W, NT, kRG, 1, true> : lora_expand_kernel<W, NT, kRG, 1, false>)
-                                         : (vec_b ? lora_expand_kernel<W, NT, kRG, 2, true> : lora_expand_kernel<W, NT, kRG, 2, false>);
-    if (const int32_t e = allow_dynamic_smem(expand, smem, "lora_expand smem")) return e;
-    return lora_start(expand, out, smem, p, true, stream, "lora_expand_kernel");
+    // Registers for two units ahead, or for twice the rows.
+    return p.max_rank <= 16 ? lora_expand<W, NT, NT == 1 ? 2 : 1, 1>(p, ctas(lora_ceil(p.rows, kLoraWarps * kLoraRows)), smem, vec_b, stream)
+                            : lora_expand<W, NT, 1, sizeof(W) == 4 ? 1 : 2>(p, ctas(lora_ceil(p.rows, kLoraWarps * kLoraRows)), smem, vec_b, stream);
 }
 
 }  // namespace
