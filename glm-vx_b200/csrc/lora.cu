@@ -84,6 +84,27 @@ __device__ __forceinline__ LoraRaw<W> lora_load4(const W *w, int n) {
     return raw;
 }
 
+// Eight neighbouring values (with VEC on their 16-byte boundary), read where n > 0; without VEC those from n on are 0.
+template <class W>
+struct LoraEight {
+    LoraRaw<W> q[2];
+};
+
+template <class W, bool VEC>
+__device__ __forceinline__ LoraEight<W> lora_load8(const W *w, int n) {
+    LoraEight<W> v{};
+    if constexpr (VEC && sizeof(W) == 2) {
+        if (n > 0) {
+            const uint4 u = __ldg(reinterpret_cast<const uint4 *>(w));
+            v.q[0] = make_uint2(u.x, u.y), v.q[1] = make_uint2(u.z, u.w);
+        }
+    } else {
+        v.q[0] = lora_load4<W, VEC>(w, n);
+        v.q[1] = lora_load4<W, VEC>(w + 4, n - 4);
+    }
+    return v;
+}
+
 // Keeps the first n of the four values (n <= 0: none).
 template <class W>
 __device__ __forceinline__ LoraRaw<W> lora_mask(int n) {
@@ -297,14 +318,14 @@ __global__ void __launch_bounds__(kLoraPlanThreads) lora_plan_kernel(LoraArgs p,
 // what they make is a column or a row of the tile that nobody keeps.
 template <class W, int MT, int MW, int NT, bool VEC>
 __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(LoraArgs p) {
-    constexpr int kUnits = 2, kKWarps = kLoraWarps / MW, kRanks = 16 * MT * MW, kStride = 8 * NT + 1;
-    constexpr int kBatch = 16 * kUnits * kKWarps;  // columns from a warp's units to its next
+    constexpr int kKWarps = kLoraWarps / MW, kRanks = 16 * MT * MW, kStride = 8 * NT + 1;
+    constexpr int kBatch = 32 * kKWarps;  // columns from a warp's block to its next
     __shared__ LoraTiles<8 * NT> tiles;
     __shared__ float parts[kKWarps][kRanks * kStride];
     grid_dependency_wait();  // the plan comes from the kernel before
     allow_dependent_launch();
     lora_tiles(tiles, p, blockIdx.x == 0);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = 4 * (lane & 3);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = 4 * (lane & 3), t8 = 2 * t4;
     const int chunks = (p.max_rank + kRanks - 1) / kRanks, per_tile = p.splits * chunks;
     for (int64_t item = blockIdx.x; item < static_cast<int64_t>(tiles.count) * per_tile; item += gridDim.x) {
     lora_open(tiles, p, static_cast<int>(item / per_tile));
@@ -312,58 +333,51 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(LoraArgs p
     const int a = tiles.adapter, n = tiles.n, rank = lora_rank(p, a);
     if (r0 >= rank) continue;
     const int kw = warp / MW, rw = r0 + 16 * MT * (warp % MW) + g;  // the lane's first rank
-    const int u0 = split * p.units + kUnits * kw, u1 = min((split + 1) * p.units, (p.cols + 15) / 16);
+    const int u0 = split * p.units + 2 * kw, u1 = min((split + 1) * p.units, (p.cols + 15) / 16);
     const W *w[2 * MT];
     const float *x[NT];
 #pragma unroll
     for (int i = 0; i < 2 * MT; ++i) {
         const int r = rw + 8 * i < rank ? rw + 8 * i : 0;
-        w[i] = static_cast<const W *>(p.a) + (static_cast<int64_t>(a) * p.max_rank + r) * p.cols + 16 * u0 + t4;
+        w[i] = static_cast<const W *>(p.a) + (static_cast<int64_t>(a) * p.max_rank + r) * p.cols + 16 * u0 + t8;
     }
 #pragma unroll
-    for (int j = 0; j < NT; ++j) x[j] = p.x + tiles.tokens[8 * j + g] * p.x_stride + 16 * u0 + t4;
+    for (int j = 0; j < NT; ++j) x[j] = p.x + tiles.tokens[8 * j + g] * p.x_stride + 16 * u0 + t8;
     float acc[MT][NT][4] = {};
     struct Batch {
-        LoraRaw<W> w[kUnits][2 * MT];
-        uint4 x[kUnits][NT];
+        LoraEight<W> w[2 * MT];
+        LoraEight<float> x[NT];
     };
     const auto load = [&](Batch &t, int left) {  // left: columns from the lane's first to the end of the split
 #pragma unroll
-        for (int k = 0; k < kUnits; ++k) {
+        for (int j = 0; j < NT; ++j) t.x[j] = lora_load8<float, VEC>(x[j], left), x[j] += kBatch;
 #pragma unroll
-            for (int j = 0; j < NT; ++j) t.x[k][j] = lora_load4<float, VEC>(x[j] + 16 * k, left - 16 * k);
-#pragma unroll
-            for (int i = 0; i < 2 * MT; ++i) t.w[k][i] = lora_load4<W, VEC>(w[i] + 16 * k, left - 16 * k);
-        }
-#pragma unroll
-        for (int j = 0; j < NT; ++j) x[j] += kBatch;
-#pragma unroll
-        for (int i = 0; i < 2 * MT; ++i) w[i] += kBatch;
+        for (int i = 0; i < 2 * MT; ++i) t.w[i] = lora_load8<W, VEC>(w[i], left), w[i] += kBatch;
     };
     const auto multiply = [&](const Batch &t) {
 #pragma unroll
-        for (int k = 0; k < kUnits; ++k) {
+        for (int k = 0; k < 2; ++k) {
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
                 uint32_t hi[4], lo[4];
-                lora_split(lora_f32<float>(t.x[k][j]), hi, lo);
+                lora_split(lora_f32<float>(t.x[j].q[k]), hi, lo);
 #pragma unroll
                 for (int i = 0; i < MT; ++i)
-                    lora_unit<sizeof(W) == 4>(acc[i][j], lora_f32<W>(t.w[k][2 * i]), lora_f32<W>(t.w[k][2 * i + 1]), hi,
-                                              lo);
+                    lora_unit<sizeof(W) == 4>(acc[i][j], lora_f32<W>(t.w[2 * i].q[k]), lora_f32<W>(t.w[2 * i + 1].q[k]),
+                                              hi, lo);
             }
         }
     };
     Batch even, odd;
-    int left = min(p.cols, 16 * u1) - (16 * u0 + t4);
-    // left + t4 is what the warp's first lane has left: the same in all lanes
+    int left = min(p.cols, 16 * u1) - (16 * u0 + t8);
+    // left + t8 is what the warp's first lane has left: the same in all lanes
     load(even, left);
-    while (left + t4 > 0) {
-        if (left + t4 > kBatch) load(odd, left - kBatch);
+    while (left + t8 > 0) {
+        if (left + t8 > kBatch) load(odd, left - kBatch);
         multiply(even);
-        if (left + t4 <= kBatch) break;
+        if (left + t8 <= kBatch) break;
         left -= 2 * kBatch;
-        if (left + t4 > 0) load(even, left);
+        if (left + t8 > 0) load(even, left);
         multiply(odd);
     }
     // acc[i][j]: ranks rw + 16 i (+ 8), tokens 8 j + t4 / 2 (+ 1)
@@ -412,12 +426,15 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(LoraArgs p
         const int first = static_cast<int>(at % per_tile);
         const int steps = static_cast<int>(min(end - at, static_cast<int64_t>(per_tile - first)));
         at += steps;
-        const int a = tiles.adapter, n = tiles.n, rank = lora_rank(p, a), units = (rank + 15) / 16;
+        const int a = tiles.adapter, n = tiles.n, rank = lora_rank(p, a);
+        constexpr int kChunk = 16 * KU;
+        const int chunks = (rank + kChunk - 1) / kChunk, lane_r = KU * t4;  // a lane has 4 KU neighbouring ranks of a chunk
         if (rank == 0) continue;
-        const int pitch = 16 * (units | 1);  // 16 mod 32 banks: the quarters of a warp's 16-byte reads do not meet
+        // 16 or 4 mod 32 banks: the quarters of a warp's 16-byte reads do not meet
+        const int pitch = KU == 1 ? 16 * (chunks | 1) : kChunk * chunks + 4;
         const float scale = p.scales[a];
         float *ls = hs + 8 * NT * pitch;
-        const W *b = static_cast<const W *>(p.b) + static_cast<int64_t>(a) * p.rows * p.max_rank + t4;
+        const W *b = static_cast<const W *>(p.b) + static_cast<int64_t>(a) * p.rows * p.max_rank + lane_r;
         float *y[NT][2];  // the lane's tokens' rows
         bool mine[NT][2];
 #pragma unroll
@@ -454,18 +471,18 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(LoraArgs p
                 }
             }
         };
-        const auto load_w = [&](Weights &to, int row, int u) {
+        const auto load_w = [&](Weights &to, int row, int c) {
 #pragma unroll
             for (int q = 0; q < RG; ++q) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int r = min(row + kLoraRows * q + i, VEC ? p.rows - 4 + i : p.rows - 1);
-                    const W *from = b + static_cast<int64_t>(r) * p.max_rank;
-#pragma unroll
-                    for (int k = 0; k < KU; ++k) {
-                        const int c = 16 * min(u + k, units - 1);
-                        if (VEC) to.w[k][q][i] = t4 + c < rank ? __ldg(reinterpret_cast<const LoraRaw<W> *>(from + c)) : LoraRaw<W>{};
-                        else to.w[k][q][i] = lora_load4<W, false>(from + c, rank - c - t4);
+                    const int r = min(row + kLoraRows * q + i, VEC ? p.rows - 4 + i : p.rows - 1), left = rank - kChunk * c - lane_r;
+                    const W *from = b + static_cast<int64_t>(r) * p.max_rank + kChunk * c;
+                    if constexpr (KU == 2) {
+                        const LoraEight<W> v = lora_load8<W, VEC>(from, left);
+                        to.w[0][q][i] = v.q[0], to.w[1][q][i] = v.q[1];
+                    } else {
+                        to.w[0][q][i] = lora_load4<W, VEC>(from, left);
                     }
                 }
             }
@@ -478,8 +495,8 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(LoraArgs p
         // h, its parts joined in order, as hi + lo; zero behind the rank
         if (!waited) grid_dependency_wait();  // h comes from the kernel before
         waited = true;
-        for (int i = tid; i < 8 * NT * 16 * units; i += kLoraThreads) {
-            const int tok = i / (16 * units), r = i - tok * 16 * units;
+        for (int i = tid; i < 8 * NT * kChunk * chunks; i += kLoraThreads) {
+            const int tok = i / (kChunk * chunks), r = i - tok * kChunk * chunks;
             float sum = 0.0f;
             if (tok < n && r < rank) {
                 const float *h = p.h + static_cast<int64_t>(tiles.tokens[tok]) * p.max_rank + r;
@@ -497,26 +514,27 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(LoraArgs p
             ls[tok * pitch + r] = __uint_as_float(lora_tf32(sum - __uint_as_float(hi)));
         }
         __syncthreads();
-        const LoraRaw<W> last_mask = lora_mask<W>(rank - 16 * (units - 1) - t4);
+        LoraRaw<W> last_mask[KU];
+#pragma unroll
+        for (int k = 0; k < KU; ++k) last_mask[k] = lora_mask<W>(rank - kChunk * (chunks - 1) - lane_r - 4 * k);
         for (int step = 0; step < steps; ++step, row += kNext) {
             if (step + 1 < steps) load_y(next, row + kNext);
             float acc[RG][2][NT][4] = {};
-            for (int u = 0; u < units; u += KU) {
-                if (u + KU < units) load_w(ahead, row, u + KU);
+            for (int c = 0; c < chunks; ++c) {
+                if (c + 1 < chunks) load_w(ahead, row, c + 1);
                 else if (step + 1 < steps) load_w(ahead, row + kNext, 0);
 #pragma unroll
                 for (int k = 0; k < KU; ++k) {
-                    if (u + k >= units) break;
-                    if (u + k == units - 1) {
+                    if (c == chunks - 1) {
 #pragma unroll
                         for (int q = 0; q < RG; ++q) {
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) lora_keep(wt.w[k][q][i], last_mask);
+                            for (int i = 0; i < 4; ++i) lora_keep(wt.w[k][q][i], last_mask[k]);
                         }
                     }
 #pragma unroll
                     for (int j = 0; j < NT; ++j) {
-                        const int from = (8 * j + g) * pitch + 16 * (u + k) + t4;
+                        const int from = (8 * j + g) * pitch + kChunk * c + lane_r + 4 * k;
                         const uint4 h4 = *reinterpret_cast<const uint4 *>(hs + from);
                         const uint4 l4 = *reinterpret_cast<const uint4 *>(ls + from);
                         const uint32_t hi[4] = {h4.x, h4.y, h4.z, h4.w}, lo[4] = {l4.x, l4.y, l4.z, l4.w};
@@ -611,7 +629,9 @@ int32_t lora_shrink(const LoraArgs &p, dim3 grid, bool vec, cudaStream_t stream)
 }
 
 template <class W, int NT, int RG, int KU>
-int32_t lora_expand(const LoraArgs &p, dim3 grid, size_t smem, bool vec, cudaStream_t stream) {
+int32_t lora_expand(const LoraArgs &p, dim3 grid, bool vec, cudaStream_t stream) {
+    const int chunks = lora_ceil(p.max_rank, 16 * KU), pitch = KU == 1 ? 16 * (chunks | 1) : 32 * chunks + 4;
+    const size_t smem = sizeof(float) * 2 * 8 * NT * pitch;
     const auto kernel = vec ? lora_expand_kernel<W, NT, RG, KU, true> : lora_expand_kernel<W, NT, RG, KU, false>;
     if (const int32_t rc = allow_dynamic_smem(kernel, smem, "lora_expand smem")) return rc;
     return lora_start(kernel, grid, smem, p, true, stream, "lora_expand_kernel");
@@ -627,9 +647,9 @@ int32_t lora_launch(LoraArgs &p, bool vec_a, bool vec_b, cudaStream_t stream) {
         lora_plan_kernel<<<1, kLoraPlanThreads, 0, stream>>>(p, 8 * NT);
         if (const int32_t rc = launch_status("lora_plan_kernel")) return rc;
     }
-    // Columns in as many parts as give four items an SM were every tile full, none shorter than four units a warp.
+    // Columns in as many parts as give two items an SM were every tile full, none shorter than four units a warp.
     const int full = lora_ceil(p.tokens, 8 * NT), all_units = lora_ceil(p.cols, 16);
-    p.splits = std::min({lora_max_splits(p.tokens), lora_ceil(all_units, 4 * kLoraWarps), lora_ceil(4 * sms, full)});
+    p.splits = std::clamp(2 * sms / full, 1, std::min(lora_max_splits(p.tokens), lora_ceil(all_units, 4 * kLoraWarps)));
     p.units = lora_ceil(all_units, p.splits);
     p.splits = lora_ceil(all_units, p.units);
     const int ranks = p.max_rank <= 16 ? 16 : p.max_rank <= 32 ? 32 : kLoraRankChunk;
@@ -641,10 +661,11 @@ int32_t lora_launch(LoraArgs &p, bool vec_a, bool vec_b, cudaStream_t stream) {
     else if (ranks == 32) rc = lora_shrink<W, 2, 1, NT>(p, grid, vec_a, stream);
     else rc = lora_shrink<W, 2, 2, NT>(p, grid, vec_a, stream);
     if (rc) return rc;
-    const size_t smem = sizeof(float) * 2 * 8 * NT * 16 * (lora_ceil(p.max_rank, 16) | 1);
-    // Registers for two units ahead, or for twice the rows.
-    return p.max_rank <= 16 ? lora_expand<W, NT, NT == 1 ? 2 : 1, 1>(p, ctas(lora_ceil(p.rows, kLoraWarps * kLoraRows)), smem, vec_b, stream)
-                            : lora_expand<W, NT, 1, sizeof(W) == 4 ? 1 : 2>(p, ctas(lora_ceil(p.rows, kLoraWarps * kLoraRows)), smem, vec_b, stream);
+    // Ranks a chunk: 16, with twice the rows a step for single tokens, or 32.
+    const dim3 out = ctas(lora_ceil(p.rows, kLoraWarps * kLoraRows));
+    if (sizeof(W) == 4 || p.max_rank <= 16)
+        return lora_expand<W, NT, NT == 1 && sizeof(W) == 2 ? 2 : 1, 1>(p, out, vec_b, stream);
+    return lora_expand<W, NT, 1, sizeof(W) == 4 ? 1 : 2>(p, out, vec_b, stream);
 }
 
 }  // namespace
@@ -695,11 +716,11 @@ GLMVX_EXPORT int32_t glmvx_lora_add(float *y, int64_t y_stride, const float *x, 
         p.counts = reinterpret_cast<int *>(ws + layout.counts);
         p.ntiles = reinterpret_cast<int *>(ws + layout.ntiles);
     }
-    // Four neighbours at once where they stand on their boundary.
-    const int four = kind == 0 ? 15 : 7;
-    const bool vec_a = !(cols & 3) && !(bits(a) & four) && !(bits(x) & 15) && (tokens == 1 || !(x_stride & 3));
-    const bool vec_b = !(max_rank & 3) && !(rows & 3) && !(bits(b) & four) && !(bits(y) & 15) &&
-                       (tokens == 1 || !(y_stride & 3));
+    // 16 bytes at once (8 for ranks up to 16) where they stand on their boundary.
+    const int per_a = kind == 0 ? 4 : 8, per_b = kind == 0 || max_rank <= 16 ? 4 : 8;
+    const bool vec_a = !(cols % per_a) && !((bits(a) | bits(x)) & 15) && (tokens == 1 || !(x_stride & 3));
+    const bool vec_b = !(max_rank % per_b) && !(rows & 3) && !(bits(b) & (kind == 0 || per_b == 8 ? 15 : 7)) &&
+                       !(bits(y) & 15) && (tokens == 1 || !(y_stride & 3));
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool wide = tokens > kLoraScan;
     if (kind == 0) return wide ? lora_launch<float, 2>(p, vec_a, vec_b, s) : lora_launch<float, 1>(p, vec_a, vec_b, s);
