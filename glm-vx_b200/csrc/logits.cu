@@ -156,8 +156,9 @@ __global__ void __launch_bounds__(kSelThreads, 2) logits_select_kernel(SelArgs p
         for (int e = 0; e < 4; ++e) k |= (__shfl_sync(0xffffffffu, word, e) >> lane & 1u) << e;
         return k;
     };
-    // Entries: the biases, then (with penalties) the history and the fed token.
-    const int entries = biases + (p.penalties && (len > 0 || fed >= 0) ? len + 1 : 0);
+    // Entries: the biases, then (with penalties that do something) the history and the fed token.
+    const bool neutral = rep == 1.0f && pres == 0.0f && freq == 0.0f;  // changes no logit, whatever was said
+    const int entries = biases + (!neutral && (len > 0 || fed >= 0) ? len + 1 : 0);
     const auto entry_id = [&](int j) {
         return j >= entries ? -1 : j < biases ? bias_ids[j] : j - biases < len ? history[j - biases] : fed;
     };

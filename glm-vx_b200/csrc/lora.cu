@@ -322,84 +322,84 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(LoraArgs p
     constexpr int kBatch = 32 * kKWarps;  // columns from a warp's block to its next
     __shared__ LoraTiles<8 * NT> tiles;
     __shared__ float parts[kKWarps][kRanks * kStride];
+    struct Batch {
+        LoraEight<W> w[2 * MT];
+        LoraEight<float> x[NT];
+    };
     grid_dependency_wait();  // the plan comes from the kernel before
     allow_dependent_launch();
     lora_tiles(tiles, p, blockIdx.x == 0);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = 4 * (lane & 3), t8 = 2 * t4;
     const int chunks = (p.max_rank + kRanks - 1) / kRanks, per_tile = p.splits * chunks;
     for (int64_t item = blockIdx.x; item < static_cast<int64_t>(tiles.count) * per_tile; item += gridDim.x) {
-    lora_open(tiles, p, static_cast<int>(item / per_tile));
-    const int part = static_cast<int>(item % per_tile), split = part / chunks, r0 = part % chunks * kRanks;
-    const int a = tiles.adapter, n = tiles.n, rank = lora_rank(p, a);
-    if (r0 >= rank) continue;
-    const int kw = warp / MW, rw = r0 + 16 * MT * (warp % MW) + g;  // the lane's first rank
-    const int u0 = split * p.units + 2 * kw, u1 = min((split + 1) * p.units, (p.cols + 15) / 16);
-    const W *w[2 * MT];
-    const float *x[NT];
+        lora_open(tiles, p, static_cast<int>(item / per_tile));
+        const int part = static_cast<int>(item % per_tile), split = part / chunks, r0 = part % chunks * kRanks;
+        const int a = tiles.adapter, n = tiles.n, rank = lora_rank(p, a);
+        if (r0 >= rank) continue;
+        const int kw = warp / MW, rw = r0 + 16 * MT * (warp % MW) + g;  // the lane's first rank
+        const int u0 = split * p.units + 2 * kw, u1 = min((split + 1) * p.units, (p.cols + 15) / 16);
+        const W *w[2 * MT];
+        const float *x[NT];
 #pragma unroll
-    for (int i = 0; i < 2 * MT; ++i) {
-        const int r = rw + 8 * i < rank ? rw + 8 * i : 0;
-        w[i] = static_cast<const W *>(p.a) + (static_cast<int64_t>(a) * p.max_rank + r) * p.cols + 16 * u0 + t8;
-    }
+        for (int i = 0; i < 2 * MT; ++i) {
+            const int r = rw + 8 * i < rank ? rw + 8 * i : 0;
+            w[i] = static_cast<const W *>(p.a) + (static_cast<int64_t>(a) * p.max_rank + r) * p.cols + 16 * u0 + t8;
+        }
 #pragma unroll
-    for (int j = 0; j < NT; ++j) x[j] = p.x + tiles.tokens[8 * j + g] * p.x_stride + 16 * u0 + t8;
-    float acc[MT][NT][4] = {};
-    struct Batch {
-        LoraEight<W> w[2 * MT];
-        LoraEight<float> x[NT];
-    };
-    const auto load = [&](Batch &t, int left) {  // left: columns from the lane's first to the end of the split
+        for (int j = 0; j < NT; ++j) x[j] = p.x + tiles.tokens[8 * j + g] * p.x_stride + 16 * u0 + t8;
+        float acc[MT][NT][4] = {};
+        const auto load = [&](Batch &t, int left) {  // left: columns from the lane's first to the end of the split
 #pragma unroll
-        for (int j = 0; j < NT; ++j) t.x[j] = lora_load8<float, VEC>(x[j], left), x[j] += kBatch;
+            for (int j = 0; j < NT; ++j) t.x[j] = lora_load8<float, VEC>(x[j], left), x[j] += kBatch;
 #pragma unroll
-        for (int i = 0; i < 2 * MT; ++i) t.w[i] = lora_load8<W, VEC>(w[i], left), w[i] += kBatch;
-    };
-    const auto multiply = [&](const Batch &t) {
+            for (int i = 0; i < 2 * MT; ++i) t.w[i] = lora_load8<W, VEC>(w[i], left), w[i] += kBatch;
+        };
+        const auto multiply = [&](const Batch &t) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
+            for (int k = 0; k < 2; ++k) {
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    uint32_t hi[4], lo[4];
+                    lora_split(lora_f32<float>(t.x[j].q[k]), hi, lo);
+#pragma unroll
+                    for (int i = 0; i < MT; ++i)
+                        lora_unit<sizeof(W) == 4>(acc[i][j], lora_f32<W>(t.w[2 * i].q[k]), lora_f32<W>(t.w[2 * i + 1].q[k]),
+                                                  hi, lo);
+                }
+            }
+        };
+        Batch even, odd;
+        int left = min(p.cols, 16 * u1) - (16 * u0 + t8);
+        // left + t8 is what the warp's first lane has left: the same in all lanes
+        load(even, left);
+        while (left + t8 > 0) {
+            if (left + t8 > kBatch) load(odd, left - kBatch);
+            multiply(even);
+            if (left + t8 <= kBatch) break;
+            left -= 2 * kBatch;
+            if (left + t8 > 0) load(even, left);
+            multiply(odd);
+        }
+        // acc[i][j]: ranks rw + 16 i (+ 8), tokens 8 j + t4 / 2 (+ 1)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-                uint32_t hi[4], lo[4];
-                lora_split(lora_f32<float>(t.x[j].q[k]), hi, lo);
-#pragma unroll
-                for (int i = 0; i < MT; ++i)
-                    lora_unit<sizeof(W) == 4>(acc[i][j], lora_f32<W>(t.w[2 * i].q[k]), lora_f32<W>(t.w[2 * i + 1].q[k]),
-                                              hi, lo);
+                float *at = parts[kw] + (rw - r0 + 16 * i) * kStride + 8 * j + t4 / 2;
+                at[0] = acc[i][j][0], at[1] = acc[i][j][1];
+                at[8 * kStride] = acc[i][j][2], at[8 * kStride + 1] = acc[i][j][3];
             }
         }
-    };
-    Batch even, odd;
-    int left = min(p.cols, 16 * u1) - (16 * u0 + t8);
-    // left + t8 is what the warp's first lane has left: the same in all lanes
-    load(even, left);
-    while (left + t8 > 0) {
-        if (left + t8 > kBatch) load(odd, left - kBatch);
-        multiply(even);
-        if (left + t8 <= kBatch) break;
-        left -= 2 * kBatch;
-        if (left + t8 > 0) load(even, left);
-        multiply(odd);
-    }
-    // acc[i][j]: ranks rw + 16 i (+ 8), tokens 8 j + t4 / 2 (+ 1)
+        __syncthreads();
+        const int ranks = min(kRanks, rank - r0);
+        for (int i = tid; i < n * kRanks; i += kLoraThreads) {
+            const int tok = i / kRanks, r = i % kRanks;
+            if (r >= ranks) continue;
+            float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            float *at = parts[kw] + (rw - r0 + 16 * i) * kStride + 8 * j + t4 / 2;
-            at[0] = acc[i][j][0], at[1] = acc[i][j][1];
-            at[8 * kStride] = acc[i][j][2], at[8 * kStride + 1] = acc[i][j][3];
+            for (int v = 0; v < kKWarps; ++v) sum += parts[v][r * kStride + tok];
+            p.h[(static_cast<int64_t>(split) * p.tokens + tiles.tokens[tok]) * p.max_rank + r0 + r] = sum;
         }
-    }
-    __syncthreads();
-    const int ranks = min(kRanks, rank - r0);
-    for (int i = tid; i < n * kRanks; i += kLoraThreads) {
-        const int tok = i / kRanks, r = i % kRanks;
-        if (r >= ranks) continue;
-        float sum = 0.0f;
-#pragma unroll
-        for (int v = 0; v < kKWarps; ++v) sum += parts[v][r * kStride + tok];
-        p.h[(static_cast<int64_t>(split) * p.tokens + tiles.tokens[tok]) * p.max_rank + r0 + r] = sum;
-    }
     }
 }
 

@@ -38,6 +38,7 @@ import math
 import numpy as np
 
 from . import runtime as rt
+from .adapters import projection_shapes
 from kernels.packed import LAYOUTS
 
 
@@ -116,9 +117,16 @@ class ResidentDecoder:
     moe_layer_factory (optional): callable(layer_index, loader) returning an
     object with forward_device(y, x, tokens, ids=None, weights=None) for the
     sparse layers (e.g. an expert-parallel layer); default: the whole layer
-    on this GPU (glmvx_moe_ffn)."""
+    on this GPU (glmvx_moe_ffn).
+    adapters (optional): an AdapterBank (gpu/adapters.py) whose projections
+    are added to this model's, each sequence by the adapter that set_adapter
+    gave it (none at first).  The bank stays the caller's to close.
+    rules (optional): a LogitRules (gpu/rules.py) of this batch and
+    vocabulary; a step's logits are then the ones its rules leave, and the
+    chosen token is -1 where they leave nothing."""
 
-    def __init__(self, backend, config, source, batch, capacity, layers=None, moe_layer_factory=None):
+    def __init__(self, backend, config, source, batch, capacity, layers=None, moe_layer_factory=None, adapters=None,
+                 rules=None):
         self.backend, self.lib = backend, backend.lib
         c = self.config = dict(config)
         self.n_layers = int(layers if layers is not None else c['num_hidden_layers'])
@@ -141,6 +149,17 @@ class ResidentDecoder:
         self.indexer_types, self.mlp_types = self.indexer_types[:self.n_layers], self.mlp_types[:self.n_layers]
         if self.indexer_types[0] != 'full':
             raise ValueError('the first layer must have a full indexer')
+        if rules is not None and (rules.batch, rules.vocab) != (self.B, self.vocab):
+            raise ValueError(f'rules are for {rules.batch} sequences over {rules.vocab} tokens, '
+                             f'not {self.B} over {self.vocab}')
+        if adapters is not None:
+            shapes = projection_shapes(c, self.n_layers)
+            for name, shape in adapters.shapes.items():
+                if shapes.get(name) != shape:
+                    raise ValueError(f'{name} {shape} is not a projection of this model that adapters may change')
+            if adapters.max_tokens < self.B:
+                raise ValueError('the adapter bank was made for fewer sequences')
+        self.adapters, self.rules = adapters, rules
         self._bufs = []
         self._moe_factory = moe_layer_factory
         self._synthetic = isinstance(source, SyntheticWeights)
@@ -310,6 +329,8 @@ class ResidentDecoder:
         self.act = self._dev(f * B * I).ptr
         self.logits = self._dev(f * B * self.vocab).ptr
         self.tokens = self._dev(4 * B).ptr
+        self.adapter_ids = self._dev(4 * B)
+        rt.call('glmvx_memset', self.adapter_ids.ptr, 0xff, 4 * B, self.s)  # -1: none
         self.full = self._dev(4).ptr
         for L, t in zip(self.layers, self.indexer_types):
             L['latents'] = self._dev(f * B * cap * self.rank).ptr
@@ -333,12 +354,15 @@ class ResidentDecoder:
     def _check(self, code, name):
         rt.check(self.lib, code, name)
 
-    def _linear(self, out, x, w):
+    def _linear(self, out, x, w, name=None):
+        """out = W x for the batch, plus the adapters' change of projection `name`."""
         ptr, kind, rows, cols = w
         if kind == 0:
             self._check(self.lib.glmvx_matmul_nt(out, x, ptr, self.B, rows, cols, self.s), 'glmvx_matmul_nt')
         else:
             self._check(self.lib.glmvx_packed_gemm(kind, out, ptr, x, rows, cols, self.B, self.s), 'glmvx_packed_gemm')
+        if self.adapters is not None and name in self.adapters.shapes:
+            self.adapters.add(name, out, x, self.adapter_ids.ptr, self.B, self.s)
 
     def _rmsnorm(self, out, x, w, n, eps, x_stride=None):
         self._check(self.lib.glmvx_rmsnorm_rows(out, x, w, self.B, n, x_stride or n, n, eps, self.s),
@@ -353,10 +377,11 @@ class ResidentDecoder:
         B, H, R, P, N, V = self.B, self.hidden, self.rank, self.rot, self.nope, self.vdim
         heads, IH, ID = self.heads, self.ih, self.idim
         pos = L['lens'].ptr  # cached rows per sequence = this token's position (read before the append)
-        self._linear(self.qa, self.n, L['q_a'])
+        m = f'model.layers.{i}.self_attn.'
+        self._linear(self.qa, self.n, L['q_a'], m + 'q_a_proj')
         self._rmsnorm(self.qr, self.qa, L['q_a_norm'], self.q_lora, 1e-6)
-        self._linear(self.query, self.qr, L['q_b'])
-        self._linear(self.comp, self.n, L['kv_a'])
+        self._linear(self.query, self.qr, L['q_b'], m + 'q_b_proj')
+        self._linear(self.comp, self.n, L['kv_a'], m + 'kv_a_proj_with_mqa')
         self._rmsnorm(self.new_latent, self.comp, L['kv_a_norm'], R, 1e-6, x_stride=R + P)
         self._rope(self.new_rope, self.comp, pos, 1, P, 0, R + P, 0, R, P, 0)
         full = self.indexer_types[i] == 'full'
@@ -392,19 +417,20 @@ class ResidentDecoder:
             sel = sel_prev
         self._check(self.lib.glmvx_absorb_value(self.vout, self.att, L['kvb'], B, heads, N, R, V, self.s),
                     'glmvx_absorb_value')
-        self._linear(self.ffn, self.vout, L['o'])  # attention output (ffn buffer reused)
+        self._linear(self.ffn, self.vout, L['o'], m + 'o_proj')  # attention output (ffn buffer reused)
         self._check(self.lib.glmvx_add(self.x, self.x, self.ffn, B * H, self.s), 'glmvx_add')
         return sel
 
-    def _feed_forward(self, L):
+    def _feed_forward(self, i, L):
         B, H = self.B, self.hidden
         self._rmsnorm(self.n, self.x, L['post_norm'], H, self.eps)
         if 'mlp' in L:
             gate, up, down = L['mlp']
-            self._linear(self.g, self.n, gate)
-            self._linear(self.u, self.n, up)
+            m = f'model.layers.{i}.mlp.'
+            self._linear(self.g, self.n, gate, m + 'gate_proj')
+            self._linear(self.u, self.n, up, m + 'up_proj')
             self._check(self.lib.glmvx_swiglu(self.act, self.g, self.u, B * gate[2], self.s), 'glmvx_swiglu')
-            self._linear(self.ffn, self.act, down)
+            self._linear(self.ffn, self.act, down, m + 'down_proj')
         else:
             L['moe'].forward_device(self.ffn, self.n, B)
         self._check(self.lib.glmvx_add(self.x, self.x, self.ffn, B * H, self.s), 'glmvx_add')
@@ -434,10 +460,14 @@ class ResidentDecoder:
         for i, L in enumerate(self.layers):
             self._rmsnorm(self.n, self.x, L['in_norm'], H, self.eps)
             sel = self._attention(i, L, sel)
-            self._feed_forward(L)
+            self._feed_forward(i, L)
         self._rmsnorm(self.n, self.x, self.final_norm, H, self.eps)
         self._linear(self.logits, self.n, self.lm_head)
-        self._check(self.lib.glmvx_argmax_rows(self.tokens, self.logits, B, self.vocab, self.s), 'glmvx_argmax_rows')
+        if self.rules is not None:
+            self.rules.select(self.tokens, self.logits, self.s)
+        else:
+            self._check(self.lib.glmvx_argmax_rows(self.tokens, self.logits, B, self.vocab, self.s),
+                        'glmvx_argmax_rows')
 
     # ---------------------------------------------------------------- API
     def step_graph(self):
@@ -507,15 +537,34 @@ class ResidentDecoder:
         self.check()
         return np.stack(out, axis=1), (np.stack(logits, axis=1) if with_logits else None)
 
-    def reset_slot(self, b):
-        """Empty sequence b's caches in every layer (its length to 0)."""
+    def set_adapter(self, b, slot=None):
+        """Sequence b runs with adapter `slot` of the bank from the next step on (None: with none)."""
         if not 0 <= b < self.B:
             raise ValueError('slot outside the batch')
+        if slot is not None:
+            if self.adapters is None:
+                raise ValueError('the decoder has no adapter bank')
+            if type(slot) is not int or not 0 <= slot < self.adapters.slots or not self.adapters.loaded[slot]:
+                raise ValueError('no adapter is loaded there')
+        self.backend.stream.synchronize()  # the step in flight has read the ids
+        self.adapter_ids.upload(np.array([-1 if slot is None else slot], np.int32), self.s, 4 * b)
+        self.backend.stream.synchronize()
+
+    def reset_slot(self, b):
+        """Empty sequence b's caches in every layer (its length to 0); with
+        rules, its history and its rules too."""
+        if not 0 <= b < self.B:
+            raise ValueError('slot outside the batch')
+        if self.rules is not None:
+            self.rules.clear(b)
         for L in self.layers:
             rt.call('glmvx_memset', L['lens'].ptr + 4 * b, 0, 4, self.s)
 
     def reset(self):
-        """Empty every cache (lengths to 0)."""
+        """Empty every cache (lengths to 0), and with rules every history (the
+        rules themselves stay)."""
+        if self.rules is not None:
+            self.rules.restart()
         for L in self.layers:
             rt.call('glmvx_memset', L['lens'].ptr, 0, 4 * self.B, self.s)
         rt.call('glmvx_memset', self.full, 0, 4, self.s)

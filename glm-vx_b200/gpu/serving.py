@@ -19,6 +19,14 @@ from the row's logits exactly as the reference's _sample does
 (scheduler.py:113-120).  The prefix cache and batched prefill of the
 reference are not rebuilt (a prompt runs through the decode steps, one
 token per step, which is the reference's prefill_token semantics).
+
+Beyond the reference, a request may bring its own low-rank adapter (a decoder
+with an AdapterBank, gpu/adapters.py) and its own rules for what it may say
+(a decoder with LogitRules, gpu/rules.py): penalties for repeated tokens,
+per-token biases, and a mask of allowed tokens, fixed or given anew for each
+token by a function of the tokens generated so far (a grammar).  They are
+applied on the device; a request whose rules leave no token ends with reason
+'exhausted'.
 """
 from collections import deque
 from dataclasses import dataclass, field
@@ -28,6 +36,8 @@ import time
 import uuid
 
 import numpy as np
+
+from .rules import pack_mask
 
 
 class BusyError(Exception):
@@ -53,6 +63,10 @@ class Request:
     reservation: int = 0
     slot: int = -1
     decode_seconds: float = 0.0
+    adapter: int | None = None
+    rules: dict = field(default_factory=dict)
+    allowed: object = None
+    output: list = field(default_factory=list)
 
 
 class BatchScheduler:
@@ -80,7 +94,12 @@ class BatchScheduler:
         self.thread.start()
 
     # ---------------------------------------------------------- admission
-    def submit(self, tokens, max_tokens, temperature=0.0, seed=0):
+    def submit(self, tokens, max_tokens, temperature=0.0, seed=0, *, adapter=None, repetition_penalty=1.0,
+               presence_penalty=0.0, frequency_penalty=0.0, logit_bias=None, allowed=None):
+        """adapter: a loaded slot of the decoder's bank.  logit_bias: {token:
+        value to add, -inf to ban}.  allowed: the tokens that may be said, as a
+        boolean array over the vocabulary or token ids, or a function from
+        the list of tokens generated so far to such a mask (or None: all)."""
         cfg = self.config
         if not isinstance(tokens, list) or not tokens or any(type(t) is not int or not 0 <= t < cfg['vocab_size']
                                                              for t in tokens):
@@ -92,10 +111,15 @@ class BatchScheduler:
             raise ValueError('temperature must be finite and nonnegative')
         if type(seed) is not int or seed < 0:
             raise ValueError('seed must be a nonnegative integer')
+        rules = self._rules(repetition_penalty, presence_penalty, frequency_penalty, logit_bias, allowed)
+        if adapter is not None:
+            bank = getattr(self.decoder, 'adapters', None)
+            if bank is None or type(adapter) is not int or not 0 <= adapter < bank.slots or not bank.loaded[adapter]:
+                raise ValueError('adapter must be a loaded slot of the decoder\'s adapter bank')
         amount = len(tokens) + max_tokens
         if amount > min(cfg.get('max_position_embeddings', 2**31 - 1), self.decoder.capacity):
             raise ValueError('request exceeds context limit')
-        req = Request(tuple(tokens), max_tokens, float(temperature), seed)
+        req = Request(tuple(tokens), max_tokens, float(temperature), seed, adapter=adapter, rules=rules, allowed=allowed)
         req.reservation = amount
         req.rng = np.random.default_rng(seed)
         req.events = queue.Queue(maxsize=min(max_tokens + 2, self.max_pending_events))
@@ -109,6 +133,34 @@ class BatchScheduler:
             self.pending.append(req)
             self.lock.notify()
         return req
+
+    def _rules(self, repetition, presence, frequency, bias, allowed):
+        """The request's rules as LogitRules.set takes them ({}: none)."""
+        rules = getattr(self.decoder, 'rules', None)
+        numbers = {'repetition_penalty': repetition, 'presence_penalty': presence, 'frequency_penalty': frequency}
+        for name, value in numbers.items():
+            if not isinstance(value, (int, float)) or isinstance(value, bool) or not np.isfinite(np.float32(value)):
+                raise ValueError(f'{name} must be finite')
+        if not np.float32(repetition) > 0:
+            raise ValueError('repetition_penalty must be positive')
+        bias = dict(bias or {})
+        vocab = self.config['vocab_size']
+        for token, value in bias.items():
+            if type(token) is not int or not 0 <= token < vocab:
+                raise ValueError('logit_bias must name valid token IDs')
+            if not isinstance(value, (int, float)) or isinstance(value, bool) or np.isnan(value) or \
+                    np.float32(value) == np.inf:
+                raise ValueError('logit_bias values must be finite or -inf')
+        if (repetition, presence, frequency) == (1.0, 0.0, 0.0) and not bias and allowed is None:
+            return {}
+        if rules is None:
+            raise ValueError('the decoder has no logit rules')
+        if len(bias) > rules.max_bias:
+            raise ValueError(f'logit_bias names more than {rules.max_bias} tokens')
+        if allowed is not None and not callable(allowed):
+            pack_mask(allowed, vocab)  # its ValueErrors now, not in the worker
+        return {'repetition': float(repetition), 'presence': float(presence), 'frequency': float(frequency),
+                'bias': bias}
 
     def cancel(self, req):
         req.cancelled.set()
@@ -150,7 +202,9 @@ class BatchScheduler:
 
     def _sample(self, logits, req):
         logits = np.asarray(logits, dtype=np.float32)
-        if logits.shape != (self.config['vocab_size'],) or not np.all(np.isfinite(logits)):
+        # a request's own rules may take tokens out (-inf); anything else that is not finite is an error
+        fine = np.isfinite(logits) | (logits == -np.inf if req.rules else False)
+        if logits.shape != (self.config['vocab_size'],) or not np.all(fine):
             raise ValueError('nonfinite or invalid logits')
         scaled = (logits.astype(np.float64) - float(np.max(logits))) / req.temperature
         probs = np.exp(scaled)
@@ -170,6 +224,14 @@ class BatchScheduler:
             self.slots[free] = req
             self.decoder.reset_slot(free)
             self.slot_len[free] = 0
+            try:
+                if getattr(self.decoder, 'adapters', None) is not None:
+                    self.decoder.set_adapter(free, req.adapter)
+                if req.rules:
+                    fixed = req.allowed if not callable(req.allowed) else None
+                    self.decoder.rules.set(free, prompt=len(req.tokens), allowed=fixed, **req.rules)
+            except ValueError as exc:  # the adapter was unloaded meanwhile, or the like: this request's own failure
+                self._finish(req, 'error', str(exc))
         for b, r in enumerate(self.slots):
             if r is None and self.slot_len[b] >= self.decoder.capacity - 1:
                 self.decoder.reset_slot(b)
@@ -186,6 +248,12 @@ class BatchScheduler:
                     self._finish(req, 'cancelled')
                 elif req.events.qsize() >= req.events.maxsize - 1:
                     self._finish(req, 'backpressure', 'client output queue is full')
+            for r in [r for r in self.slots if r is not None and callable(r.allowed)]:
+                if r.cursor + 1 >= len(r.tokens):  # the coming step's choice is used
+                    try:
+                        self.decoder.rules.allow(r.slot, r.allowed(list(r.output)))
+                    except Exception as exc:  # the request's own function failed, or its mask is none
+                        self._finish(r, 'error', str(exc))
             active = [r for r in self.slots if r is not None]
             if closed and not active:
                 return
@@ -215,7 +283,11 @@ class BatchScheduler:
                     r.cursor += 1
                     if r.cursor < len(r.tokens):
                         continue  # still inside the prompt: this step's output is not sampled
+                if r.rules and chosen[r.slot] < 0:
+                    self._finish(r, 'exhausted', 'no token is allowed')
+                    continue
                 token = self._sample(logits[r.slot], r) if r.temperature > 0 else int(chosen[r.slot])
+                r.output.append(token)
                 r.generated += 1
                 r.next_token = token
                 if r.first_token_at is None:

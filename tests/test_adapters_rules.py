@@ -1,0 +1,295 @@
+"""Adapter banks, logit rules and the scheduler's use of them, without a GPU:
+argument checks, storage rounding, masks, and the serving loop over a decoder
+that applies the rules in NumPy."""
+import numpy as np
+import pytest
+
+from gpu.adapters import AdapterBank, projection_shapes, to_kind
+from gpu.rules import LogitRules, pack_mask
+from gpu.serving import BatchScheduler, collect
+
+CONFIG = dict(num_hidden_layers=2, hidden_size=64, num_attention_heads=2, q_lora_rank=32, kv_lora_rank=32,
+              qk_nope_head_dim=16, qk_rope_head_dim=8, v_head_dim=16, intermediate_size=96, vocab_size=50,
+              mlp_layer_types=['dense', 'sparse'])
+
+
+class NoDevice:
+    """A backend whose device must not be reached."""
+    lib = None
+
+    def _begin(self):
+        raise AssertionError('the device was reached')
+
+
+def test_projection_shapes():
+    shapes = projection_shapes(CONFIG)
+    assert shapes['model.layers.0.self_attn.q_a_proj'] == (32, 64)
+    assert shapes['model.layers.1.self_attn.q_b_proj'] == (48, 32)
+    assert shapes['model.layers.0.self_attn.kv_a_proj_with_mqa'] == (40, 64)
+    assert shapes['model.layers.1.self_attn.o_proj'] == (64, 32)
+    assert shapes['model.layers.0.mlp.down_proj'] == (64, 96)
+    assert not any(name.startswith('model.layers.1.mlp') for name in shapes)
+    assert not any(name.startswith('model.layers.1') for name in projection_shapes(CONFIG, layers=1))
+
+
+@pytest.mark.parametrize('change,message', [
+    (dict(shapes={}), 'projections'), (dict(shapes={'a': (0, 4)}), 'positive'), (dict(slots=0), 'positive'),
+    (dict(max_rank=0), 'max_rank'), (dict(max_rank=257), 'max_rank'), (dict(max_tokens=0), 'positive'),
+    (dict(kind=8), 'kind')])
+def test_bank_refusals(change, message):
+    args = dict(shapes={'a': (4, 4)}, slots=2, max_rank=4, kind=30, max_tokens=4)
+    args.update(change)
+    with pytest.raises(ValueError, match=message):
+        AdapterBank(NoDevice(), **args)
+
+
+def bank_without_device():
+    bank = AdapterBank.__new__(AdapterBank)
+    bank.shapes, bank.slots, bank.max_rank, bank.kind, bank.max_tokens = {'a': (6, 4)}, 2, 3, 30, 4
+    bank.backend, bank.loaded, bank._bufs = NoDevice(), [False, False], []
+    return bank
+
+
+@pytest.mark.parametrize('slot,weights,scale,message', [
+    (2, {}, 1.0, 'slot'), (-1, {}, 1.0, 'slot'), (True, {}, 1.0, 'slot'), (0, {}, np.inf, 'scale'),
+    (0, {'b': (np.zeros((1, 4)), np.zeros((6, 1)))}, 1.0, 'not a projection'),
+    (0, {'a': (np.zeros((1, 5)), np.zeros((6, 1)))}, 1.0, 'fit'),
+    (0, {'a': (np.zeros((2, 4)), np.zeros((6, 1)))}, 1.0, 'fit'),
+    (0, {'a': (np.zeros(4), np.zeros((6, 1)))}, 1.0, 'fit'),
+    (0, {'a': (np.zeros((4, 4)), np.zeros((6, 4)))}, 1.0, 'rank 4'),
+    (0, {'a': (np.full((1, 4), np.nan), np.zeros((6, 1)))}, 1.0, 'nonfinite'),
+    (0, {'a': (np.full((1, 4), 3.4e38), np.zeros((6, 1)))}, 1.0, 'BF16')])
+def test_load_refusals(slot, weights, scale, message):
+    with pytest.raises(ValueError, match=message):
+        bank_without_device().load(slot, weights, scale)
+
+
+def test_storage_rounding():
+    x = np.array([1.0, 1 + 2.0**-8, 1 + 3 * 2.0**-8, -1 - 2.0**-8 - 2.0**-20, 2.0**-130, 0.0], np.float32)
+    got = (to_kind(x, 30).astype(np.uint32) << 16).view(np.float32)
+    assert got[:4].tolist() == [1.0, 1.0, 1 + 2.0**-6, -1 - 2.0**-7]
+    assert np.all(np.abs(got - x) <= np.abs(x) * 2.0**-8 + 2.0**-133)
+    half = to_kind(x, 1).astype(np.float32)
+    assert np.all(np.abs(half - x) <= np.abs(x) * 2.0**-11 + 2.0**-25)
+    assert to_kind(x, 0).tobytes() == x.tobytes()
+    with pytest.raises(ValueError, match='F16'):
+        to_kind(np.float32([7e4]), 1)
+
+
+def test_pack_mask():
+    keep = np.zeros(70, bool)
+    keep[[0, 31, 32, 69]] = True
+    words = pack_mask(keep, 70)
+    assert words.dtype == np.uint32 and words.tolist() == [1 | 1 << 31, 1, 1 << 5]
+    assert pack_mask([0, 31, 32, 69, 69], 70).tolist() == words.tolist()
+    assert pack_mask(np.array([69]), 70).tolist() == [0, 0, 32]
+    assert pack_mask([], 70).tolist() == [0, 0, 0] and pack_mask(set(), 70).tolist() == [0, 0, 0]
+    for bad in (np.zeros(69, bool), [70], [-1], [0.5]):
+        with pytest.raises(ValueError):
+            pack_mask(bad, 70)
+
+
+@pytest.mark.parametrize('change,message', [
+    (dict(batch=0), 'positive'), (dict(vocab=0), 'positive'), (dict(capacity=0), 'positive'),
+    (dict(max_bias=0), 'max_bias'), (dict(max_bias=2048), 'max_bias'), (dict(capacity=2**20 - 1), '2\\^20')])
+def test_rules_refusals(change, message):
+    args = dict(batch=2, vocab=10, capacity=8, max_bias=4)
+    args.update(change)
+    with pytest.raises(ValueError, match=message):
+        LogitRules(NoDevice(), **args)
+
+
+class HostRules:
+    """LogitRules' interface over NumPy."""
+
+    def __init__(self, batch, vocab):
+        self.batch, self.vocab, self.max_bias = batch, vocab, 4
+        self.rows = [None] * batch
+        for b in range(batch):
+            self.clear(b)
+
+    def clear(self, b):
+        self.rows[b] = dict(history=[], prompt=0, repetition=1.0, presence=0.0, frequency=0.0, bias={}, allowed=None)
+
+    def set(self, b, **rules):
+        self.rows[b].update(rules)
+
+    def allow(self, b, allowed):
+        if allowed is not None:
+            pack_mask(allowed, self.vocab)
+        self.rows[b]['allowed'] = allowed
+
+    def select(self, fed, logits):
+        chosen = []
+        for b, row in enumerate(self.rows):
+            row['history'].append(int(fed[b]))
+            l = logits[b].astype(np.float64)
+            for t in set(row['history']):
+                l[t] = l[t] / row['repetition'] if l[t] > 0 else l[t] * row['repetition']
+            said = row['history'][row['prompt']:]
+            for t in set(said):
+                l[t] -= said.count(t) * row['frequency'] + row['presence']
+            for t, v in row['bias'].items():
+                l[t] += v
+            if row['allowed'] is not None:
+                words = pack_mask(row['allowed'], self.vocab)
+                v = np.arange(self.vocab)
+                l[(words[v // 32] >> (v % 32).astype(np.uint32)) & 1 == 0] = -np.inf
+            logits[b] = l
+            chosen.append(int(np.argmax(l)) if l.max() > -np.inf else -1)
+        return chosen
+
+
+class HostDecoder:
+    """A decoder whose logits depend on the fed token and the sequence's adapter alone."""
+
+    def __init__(self, batch, vocab, rules=True, slots=0):
+        self.B, self.capacity, self.config = batch, 64, dict(vocab_size=vocab)
+        self.table = np.random.default_rng(3).normal(size=(4, vocab, vocab)).astype(np.float32)
+        self.rules = HostRules(batch, vocab) if rules else None
+        self.adapters = None
+        if slots:
+            self.adapters = bank_without_device()
+            self.adapters.slots, self.adapters.loaded = slots, [True] * slots
+        self.adapter = [None] * batch
+
+    def reset_slot(self, b):
+        if self.rules:
+            self.rules.clear(b)
+
+    def set_adapter(self, b, slot=None):
+        if slot is not None and not self.adapters.loaded[slot]:
+            raise ValueError('no adapter is loaded there')
+        self.adapter[b] = slot
+
+    def set_tokens(self, tokens):
+        self.fed = list(tokens)
+
+    def step(self):
+        self.logits = np.stack([self.table[0 if a is None else 1 + a, t] for a, t in zip(self.adapter, self.fed)])
+        self.chosen = self.rules.select(self.fed, self.logits) if self.rules else self.logits.argmax(1).tolist()
+
+    def read_tokens(self):
+        return np.array(self.chosen, np.int32)
+
+    def read_logits(self):
+        return self.logits.copy()
+
+
+@pytest.fixture
+def serve():
+    made = []
+
+    def start(*args, **kwargs):
+        made.append(BatchScheduler(HostDecoder(*args, **kwargs)))
+        return made[-1]
+
+    yield start
+    for sched in made:
+        sched.close()
+
+
+def greedy(table, token, n):
+    out = []
+    for _ in range(n):
+        token = int(np.argmax(table[token]))
+        out.append(token)
+    return out
+
+
+def test_requests_keep_to_their_own_rules_and_adapters(serve):
+    sched = serve(4, 50, slots=2)
+    table = sched.decoder.table
+    plain = sched.submit([7, 8], 6)
+    other = sched.submit([7, 8], 6, adapter=1)
+    first = greedy(table[0], 8, 1)[0]
+    banned = sched.submit([7, 8], 6, logit_bias={first: float('-inf')})
+    fixed = sched.submit([7, 8], 6, allowed=[3, 4])
+    assert collect(plain)[0] == greedy(table[0], 8, 6)
+    assert collect(other)[0] == greedy(table[2], 8, 6)
+    assert first not in collect(banned)[0]
+    assert set(collect(fixed)[0]) <= {3, 4}
+    again = [sched.submit([7, 8], 6) for _ in range(4)]  # the slots' rules and adapters left with their requests
+    assert all(collect(r)[0] == greedy(table[0], 8, 6) for r in again)
+
+
+def test_penalties_stop_a_loop(serve):
+    sched = serve(2, 50)
+    for t in range(50):
+        sched.decoder.table[0, t, 5] = 50.0
+        sched.decoder.table[0, t, 6] = 49.0
+    assert collect(sched.submit([1], 4))[0] == [5, 5, 5, 5]
+    assert collect(sched.submit([1], 4, frequency_penalty=0.6))[0] == [5, 5, 6, 5]
+    assert collect(sched.submit([1], 4, presence_penalty=2.0))[0] == [5, 6, 5, 5]
+    assert collect(sched.submit([5], 2, repetition_penalty=1.5))[0] == [6, 5]
+    assert collect(sched.submit([5], 2, presence_penalty=2.0))[0] == [5, 6]  # the prompt is not output
+
+
+def test_a_grammar_is_asked_before_each_token(serve):
+    sched = serve(2, 50)
+    asked = []
+
+    def grammar(output):
+        asked.append(list(output))
+        return None if len(output) == 3 else [10 + len(output)]
+
+    tokens, done = collect(sched.submit([1, 2, 3], 4, allowed=grammar))
+    assert tokens[:3] == [10, 11, 12] and done['reason'] == 'length'
+    assert asked == [[], [10], [10, 11], [10, 11, 12]]
+
+
+def test_a_request_without_a_token_left_ends_alone(serve):
+    sched = serve(2, 50)
+    fine = sched.submit([4], 5)
+    tokens, done = collect(sched.submit([4], 5, allowed=lambda output: [9] if not output else []))
+    assert tokens == [9] and done['reason'] == 'exhausted'
+    assert collect(fine)[0] == greedy(sched.decoder.table[0], 4, 5)
+
+
+@pytest.mark.parametrize('grammar', [lambda output: 1 // 0, lambda output: [50], lambda output: np.zeros(7, bool)])
+def test_a_failing_grammar_ends_its_request_alone(serve, grammar):
+    sched = serve(2, 50)
+    fine = sched.submit([4], 5)
+    tokens, done = collect(sched.submit([4], 5, allowed=grammar))
+    assert tokens == [] and done['reason'] == 'error' and done['error']
+    assert collect(fine)[0] == greedy(sched.decoder.table[0], 4, 5)
+    assert sched.status()['error'] is None and sched.status()['active_requests'] == 0
+
+
+def test_an_adapter_unloaded_before_admission_ends_its_request_alone(serve):
+    sched = serve(1, 50, slots=1)
+    hold = sched.decoder.adapters.loaded
+    with sched.lock:  # the worker admits after this block
+        req = sched.submit([4], 3, adapter=0)
+        hold[0] = False
+    assert collect(req)[1]['reason'] == 'error'
+    assert collect(sched.submit([4], 3))[0] == greedy(sched.decoder.table[0], 4, 3)
+
+
+def test_sampling_keeps_to_the_mask(serve):
+    sched = serve(1, 50)
+    tokens, _ = collect(sched.submit([4], 20, temperature=2.0, seed=5, allowed=[3, 30, 31]))
+    assert set(tokens) <= {3, 30, 31} and len(set(tokens)) > 1
+    assert collect(sched.submit([4], 20, temperature=2.0, seed=5, allowed=[3, 30, 31]))[0] == tokens
+
+
+def test_submit_refusals(serve):
+    sched = serve(1, 50, slots=2)
+    sched.decoder.adapters.loaded[1] = False
+    bad = [dict(adapter=2), dict(adapter=-1), dict(adapter=1), dict(adapter=True), dict(repetition_penalty=0),
+           dict(repetition_penalty=-1.0), dict(repetition_penalty=float('nan')), dict(presence_penalty='1'),
+           dict(frequency_penalty=float('inf')), dict(frequency_penalty=1e60), dict(logit_bias={50: 1.0}),
+           dict(logit_bias={-1: 1.0}), dict(logit_bias={True: 1.0}), dict(logit_bias={1: float('inf')}),
+           dict(logit_bias={1: float('nan')}), dict(logit_bias={i: 1.0 for i in range(5)}), dict(allowed=[50]),
+           dict(allowed=np.zeros(49, bool))]
+    for change in bad:
+        with pytest.raises(ValueError), np.errstate(over='ignore'):
+            sched.submit([1], 2, **change)
+    assert sched.status()['active_requests'] == 0
+    plain = serve(1, 50, rules=False)
+    for change in (dict(repetition_penalty=1.1), dict(logit_bias={1: 1.0}), dict(allowed=[1])):
+        with pytest.raises(ValueError, match='no logit rules'):
+            plain.submit([1], 2, **change)
+    with pytest.raises(ValueError, match='adapter'):
+        plain.submit([1], 2, adapter=0)
+    assert len(collect(plain.submit([1], 2, repetition_penalty=1, logit_bias={}))[0]) == 2
