@@ -322,6 +322,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(LoraArgs p
     constexpr int kBatch = 32 * kKWarps;  // columns from a warp's block to its next
     __shared__ LoraTiles<8 * NT> tiles;
     __shared__ float parts[kKWarps][kRanks * kStride];
+    __shared__ float4 sums[MT * NT][kLoraThreads];
     struct Batch {
         LoraEight<W> w[2 * MT];
         LoraEight<float> x[NT];
@@ -363,10 +364,28 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(LoraArgs p
                     lora_split(lora_f32<float>(t.x[j].q[k]), hi, lo);
 #pragma unroll
                     for (int i = 0; i < MT; ++i)
-                        lora_unit<sizeof(W) == 4>(acc[i][j], lora_f32<W>(t.w[2 * i].q[k]), lora_f32<W>(t.w[2 * i + 1].q[k]),
-                                                  hi, lo);
+                        lora_unit<sizeof(W) == 4>(acc[i][j], lora_f32<W>(t.w[2 * i].q[k]),
+                                                  lora_f32<W>(t.w[2 * i + 1].q[k]), hi, lo);
                 }
             }
+        };
+        // The tensor cores cut what an addition leaves over: sums through thousands of columns drift by that (2.7e-6 of
+        // the result at 6144).  Theirs end after two blocks and go on as rounded f32 sums, in the lane's own places.
+        bool begun = false;
+        const auto settle = [&]() {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    float4 &sum = sums[i * NT + j][tid];
+                    float4 v = begun ? sum : make_float4(0.f, 0.f, 0.f, 0.f);
+                    v.x += acc[i][j][0], v.y += acc[i][j][1], v.z += acc[i][j][2], v.w += acc[i][j][3];
+                    sum = v;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.0f;
+                }
+            }
+            begun = true;
         };
         Batch even, odd;
         int left = min(p.cols, 16 * u1) - (16 * u0 + t8);
@@ -379,6 +398,17 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(LoraArgs p
             left -= 2 * kBatch;
             if (left + t8 > 0) load(even, left);
             multiply(odd);
+            if (left + t8 > 0) settle();
+        }
+        if (begun) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    const float4 v = sums[i * NT + j][tid];
+                    acc[i][j][0] += v.x, acc[i][j][1] += v.y, acc[i][j][2] += v.z, acc[i][j][3] += v.w;
+                }
+            }
         }
         // acc[i][j]: ranks rw + 16 i (+ 8), tokens 8 j + t4 / 2 (+ 1)
 #pragma unroll
