@@ -714,7 +714,7 @@ GLMVX_EXPORT int32_t glmvx_lora_add(float *y, int64_t y_stride, const float *x, 
                                     const int32_t *ranks, const float *scales, int32_t tokens, int32_t rows,
                                     int32_t cols, int32_t adapters, int32_t max_rank, void *workspace,
                                     uint64_t workspace_bytes, void *stream) {
-    if (tokens < 0 || tokens > 1 << 20 || rows < 1 || cols < 1 || adapters < 1 || rows > 1 << 22)
+    if (tokens < 0 || tokens > 1 << 20 || rows < 1 || cols < 1 || adapters < 1 || rows > 1 << 22 || cols > 1 << 22)
         return set_error("lora_add: invalid dimensions"), kInvalid;
     if (max_rank < 1 || max_rank > kLoraMaxRank)
         return set_error("lora_add: max_rank must be 1..%d", kLoraMaxRank), kInvalid;

@@ -269,3 +269,21 @@ def test_captured_steps_feed_themselves(gpu_backend):
     g.close()
     for b in list(dev.values()) + [out]:
         b.close()
+
+
+@pytest.mark.parametrize('rows,vocab,cap,bias', [(1, 700001, 100000, 3), (2, 400000, 60000, 2047), (3, 1300000, 8, 1)])
+def test_vocabularies_that_go_in_passes(gpu_backend, rows, vocab, cap, bias):
+    """Histories as long as the vocabulary's share of a CTA: the rules do not fit shared memory at once."""
+    Case(rows, vocab, cap, lens=[cap, cap - 1, 0][:rows], penalties=True, bias=bias, masks=2, seed=vocab).check(gpu_backend)
+
+
+@pytest.mark.parametrize('vocab', [4, 124, 128, 132, 2048, 2052, 6148])
+def test_vocabularies_around_the_blocks(gpu_backend, vocab):
+    """One block of tokens and its neighbours, whole groups of four and not, in rows beside one another."""
+    for v in (vocab - 1, vocab):
+        Case(5, v, cap=30, penalties=True, bias=4, masks=3, pad=4 if v == vocab else 1, seed=v).check(gpu_backend, True)
+
+
+def test_many_rows(gpu_backend):
+    """More rows than run at once, each with a CTA of its own."""
+    Case(700, 1000, cap=12, penalties=True, bias=2, masks=4, seed=20).check(gpu_backend)

@@ -233,3 +233,55 @@ def test_long_rows(gpu_backend):
     Case(64, 6144, 2048, 16, 16, 30, seed=1).check(gpu_backend)
     Case(3, 576, 6144, 2, 64, 1, seed=2).check(gpu_backend)
     Case(700, 576, 2048, 3, 32, 30, ids=np.sort(np.arange(700) % 3), seed=3).check(gpu_backend)
+
+
+@pytest.mark.parametrize('kind', [0, 1, 30])
+@pytest.mark.parametrize('max_rank,cols,rows', [(8, 512, 256), (12, 520, 260), (20, 1000, 132), (24, 768, 64),
+                                                (40, 64, 1028), (64, 2056, 8), (256, 264, 36), (48, 24, 4)])
+def test_ranks_and_widths_on_both_sides_of_the_tiles(gpu_backend, kind, max_rank, cols, rows):
+    """Ranks and widths that end inside a chunk, with vector loads and without, few and many tokens."""
+    for tokens in (6, 70):
+        Case(tokens, rows, cols, 3, max_rank, kind, ids=np.arange(tokens) % 4 - 1,
+             ranks=[max_rank, max(1, max_rank // 2 + 1), 1], seed=tokens + cols).check(gpu_backend)
+
+
+def test_many_adapters_and_many_tokens(gpu_backend):
+    """More adapters than the plan counts in shared memory, more tokens than its threads keep."""
+    Case(200, 8, 16, 5000, 2, 1, seed=1).check(gpu_backend)
+    ids = np.random.default_rng(2).integers(-1, 3, 6000)
+    Case(6000, 12, 16, 3, 4, 30, ids=ids, ranks=[4, 0, 3], seed=2).check(gpu_backend)
+    Case(5000, 4, 8, 1, 1, 0, ids=np.zeros(5000), ranks=[1], seed=3).check(gpu_backend)
+
+
+def test_a_captured_call_of_many_tokens_replays(gpu_backend):
+    """The plan is made anew by each replay: ids written between two replays count in the second."""
+    case = Case(300, 64, 128, 6, 8, 30, ranks=[8] * 6, seed=9)
+    tokens, rows, cols, adapters, max_rank = case.dims
+    s, other = gpu_backend.stream, case.ids[::-1].copy()
+    need = gpu_backend.lib.glmvx_lora_workspace_bytes(tokens, adapters, max_rank)
+    bufs = {n: rt.DeviceBuffer(getattr(case, n).nbytes) for n in ('x', 'y', 'a', 'b', 'ids', 'ranks', 'scales')}
+    ws = rt.DeviceBuffer(need)
+    g = rt.Graph(s)
+    g.begin()
+    try:
+        rt.call('glmvx_lora_add', bufs['y'].ptr, rows, bufs['x'].ptr, cols, bufs['ids'].ptr, 30, bufs['a'].ptr,
+                bufs['b'].ptr, bufs['ranks'].ptr, bufs['scales'].ptr, tokens, rows, cols, adapters, max_rank, ws.ptr,
+                need, s.handle)
+    finally:
+        g.end()
+    try:
+        for n, buf in bufs.items():
+            buf.upload(getattr(case, n), s.handle)
+        first = case.run(gpu_backend)
+        for ids, start in ((case.ids, case.y), (other, first)):
+            case.ids, case.y = ids, start
+            bufs['ids'].upload(ids, s.handle)
+            g.launch()
+            got = np.empty_like(case.y)
+            bufs['y'].download(got, s.handle)
+            s.synchronize()
+            assert got.tobytes() == case.run(gpu_backend).tobytes()
+    finally:
+        g.close()
+        for buf in list(bufs.values()) + [ws]:
+            buf.close()
