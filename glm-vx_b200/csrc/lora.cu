@@ -436,9 +436,8 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(LoraArgs p
 // y[token][row] += s * B[row] . h[token] for tiles of 8 NT tokens.  A CTA's share is
 // a run of the steps of all tiles (a step: 32 RG rows a warp).  Row 4 g + i of
 // 32 stands at place g of half i of two m16 tiles, so that a lane ends up with
-// four neighbouring rows of two tokens: one float4 of y each.  y and the weights
-// (KU units of 16 ranks at once) are read one step, or KU units, ahead.  With VEC
-// lanes whose rows are behind the last read the last ones and write nothing.
+// four neighbouring rows of two tokens: one float4 of y each.  Ranks come 16 KU at a
+// time.  With VEC lanes whose rows are behind the last read the last ones and write nothing.
 template <class W, int NT, int RG, int KU, bool VEC>
 __global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(LoraArgs p) {
     extern __shared__ __align__(16) float hs[];  // [2][8 NT][pitch]: hi, lo
@@ -517,11 +516,18 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(LoraArgs p
                 }
             }
         };
-        int row = (first * kLoraWarps + warp) * kSpan + 4 * g;
-        Rows old, next;
-        Weights wt, ahead;
-        load_y(old, row);
-        load_w(wt, row, 0);
+        // A turn: a chunk of ranks of a step's rows.  The weights of two turns are on their way while a third's are
+        // multiplied; the three places take turns by name, since a copy from one to the next would wait for it.
+        int row = (first * kLoraWarps + warp) * kSpan + 4 * g, chunk = 0;
+        int fetch_row = row, fetch_chunk = 0, fetches = steps * chunks;
+        const auto fetch = [&](Weights &to) {
+            if (--fetches < 0) return;
+            load_w(to, fetch_row, fetch_chunk);
+            if (++fetch_chunk == chunks) fetch_chunk = 0, fetch_row += kNext;
+        };
+        Weights one, two, three;
+        fetch(one);
+        fetch(two);
         // h, its parts joined in order, as hi + lo; zero behind the rank
         if (!waited) grid_dependency_wait();  // h comes from the kernel before
         waited = true;
@@ -547,38 +553,41 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(LoraArgs p
         LoraRaw<W> last_mask[KU];
 #pragma unroll
         for (int k = 0; k < KU; ++k) last_mask[k] = lora_mask<W>(rank - kChunk * (chunks - 1) - lane_r - 4 * k);
-        for (int step = 0; step < steps; ++step, row += kNext) {
-            if (step + 1 < steps) load_y(next, row + kNext);
-            float acc[RG][2][NT][4] = {};
-            for (int c = 0; c < chunks; ++c) {
-                if (c + 1 < chunks) load_w(ahead, row, c + 1);
-                else if (step + 1 < steps) load_w(ahead, row + kNext, 0);
+        Rows old;
+        float acc[RG][2][NT][4];
+        const auto turn = [&](Weights &wt, Weights &later) {
+            fetch(later);
+            if (chunk == 0) {
+                load_y(old, row);
+#pragma unroll
+                for (int i = 0; i < RG * 2 * NT * 4; ++i) (&acc[0][0][0][0])[i] = 0.0f;
+            }
+            if (chunk == chunks - 1) {
 #pragma unroll
                 for (int k = 0; k < KU; ++k) {
-                    if (c == chunks - 1) {
 #pragma unroll
-                        for (int q = 0; q < RG; ++q) {
+                    for (int i = 0; i < 4 * RG; ++i) lora_keep(wt.w[k][i / 4][i % 4], last_mask[k]);
+                }
+            }
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) lora_keep(wt.w[k][q][i], last_mask[k]);
-                        }
-                    }
+            for (int k = 0; k < KU; ++k) {
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        const int from = (8 * j + g) * pitch + kChunk * c + lane_r + 4 * k;
-                        const uint4 h4 = *reinterpret_cast<const uint4 *>(hs + from);
-                        const uint4 l4 = *reinterpret_cast<const uint4 *>(ls + from);
-                        const uint32_t hi[4] = {h4.x, h4.y, h4.z, h4.w}, lo[4] = {l4.x, l4.y, l4.z, l4.w};
+                for (int j = 0; j < NT; ++j) {
+                    const int from = (8 * j + g) * pitch + kChunk * chunk + lane_r + 4 * k;
+                    const uint4 h4 = *reinterpret_cast<const uint4 *>(hs + from);
+                    const uint4 l4 = *reinterpret_cast<const uint4 *>(ls + from);
+                    const uint32_t hi[4] = {h4.x, h4.y, h4.z, h4.w}, lo[4] = {l4.x, l4.y, l4.z, l4.w};
 #pragma unroll
-                        for (int q = 0; q < RG; ++q) {
+                    for (int q = 0; q < RG; ++q) {
 #pragma unroll
-                            for (int i = 0; i < 2; ++i)
-                                lora_unit<sizeof(W) == 4>(acc[q][i][j], lora_f32<W>(wt.w[k][q][2 * i]),
-                                                          lora_f32<W>(wt.w[k][q][2 * i + 1]), hi, lo);
-                        }
+                        for (int i = 0; i < 2; ++i)
+                            lora_unit<sizeof(W) == 4>(acc[q][i][j], lora_f32<W>(wt.w[k][q][2 * i]),
+                                                      lora_f32<W>(wt.w[k][q][2 * i + 1]), hi, lo);
                     }
                 }
-                wt = ahead;
             }
+            if (++chunk < chunks) return;
+            chunk = 0;
 #pragma unroll
             for (int q = 0; q < RG; ++q) {
                 const int r = row + kLoraRows * q;
@@ -600,7 +609,12 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(LoraArgs p
                     }
                 }
             }
-            old = next;
+            row += kNext;
+        };
+        for (int left = steps * chunks; left > 0; left -= 3) {
+            turn(one, three);
+            if (left > 1) turn(two, one);
+            if (left > 2) turn(three, two);
         }
     }
     // A CTA with nothing to do must not end before the kernel before: what comes next waits for this one only.
