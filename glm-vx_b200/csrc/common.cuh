@@ -166,6 +166,12 @@ __device__ __forceinline__ void report_device_error(int *err, int code) {
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void allow_dependent_launch() { asm volatile("griddepcontrol.launch_dependents;"); }
 
+// A barrier over the CTAs of a cluster, in two halves; also orders their shared memory.
+__device__ __forceinline__ void cluster_arrive() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
 // The reference's branch-stable logistic (kernels/kernels.vx:8-15).
 __device__ __forceinline__ float sigmoid_ref(float x) {
     if (x >= 0.0f) return 1.0f / (1.0f + expf(0.0f - x));

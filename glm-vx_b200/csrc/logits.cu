@@ -68,11 +68,6 @@ __device__ __forceinline__ float sel_max(float a, float b) {
 // Whether x is an element that a row's maximum m came from.
 __device__ __forceinline__ bool sel_is(float x, float m) { return x == m || (m != m && x != x); }
 
-__device__ __forceinline__ void cluster_arrive() {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-
 // Stores v to this CTA's shared variable `at` in the CTA `rank` of the cluster.
 __device__ __forceinline__ void cluster_store(void *at, uint32_t rank, uint32_t v) {
     asm volatile(

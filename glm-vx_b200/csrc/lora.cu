@@ -3,14 +3,15 @@
 // with A_a [rank_a][cols] and B_a [rows][rank_a] taken from stacks padded to
 // max_rank.  Two kernels: lora_shrink (h = A x, f32, into the workspace, the
 // columns split over CTAs) and lora_expand (the parts of h joined, y += s B h),
-// the second launched while the first runs.
+// the second launched while the first runs; for few tiles of small adapters one
+// kernel of clusters does both.
 //
 // Both are products of a weight tile with a few tokens, bound by reading the
 // weights (few tokens an adapter) or x and y (many): tensor-core tiles whose
 // M is the weights' rows and whose N is the tokens, so that one token wastes
 // only multiplications, and every operand goes from memory straight into the
-// fragment that needs it: the order of K is free, so a lane takes four
-// neighbouring columns where the fragment layout names columns t and t + 4.
+// fragment that needs it: the order of K is free, so a lane takes eight
+// neighbouring columns where the fragment layout names t and t + 4 of each eight.
 // F16 and BF16 weights are TF32 numbers as they are; x, h and F32 weights go
 // in as two, hi + lo (x.hi, x.lo and, for F32, lo.hi products; 2^-22 of a term
 // is lost at most).  Sums are f32.
@@ -310,35 +311,31 @@ __global__ void __launch_bounds__(kLoraPlanThreads) lora_plan_kernel(LoraArgs p,
     if (tid == 0) *p.ntiles = tile_base;
 }
 
-// h[split][token][r] = A[r][the split's columns] . x[token][the split's columns]
-// for a tile of 8 NT tokens and 16 MT MW ranks, item after item.  MW warps
-// share a unit of 16 columns, 16 MT ranks each, and take every 8 / MW-th pair of
-// neighbouring units, the next pair on its way meanwhile; the warps' sums are joined in
-// order.  Lanes without a token or a rank of their own read the first one's:
+// A . x for a tile of 8 NT tokens, 16 MT MW ranks and a range of columns, by one
+// CTA.  MW warps share a block of 32 columns, 16 MT ranks each, and take every
+// 8 / MW-th block, the next one on its way meanwhile; the warps' sums are joined
+// in order.  Lanes without a token or a rank of their own read the first one's:
 // what they make is a column or a row of the tile that nobody keeps.
 template <class W, int MT, int MW, int NT, bool VEC>
-__global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(LoraArgs p) {
-    constexpr int kKWarps = kLoraWarps / MW, kRanks = 16 * MT * MW, kStride = 8 * NT + 1;
-    constexpr int kBatch = 32 * kKWarps;  // columns from a warp's block to its next
-    __shared__ LoraTiles<8 * NT> tiles;
-    __shared__ float parts[kKWarps][kRanks * kStride];
-    __shared__ float4 sums[MT * NT][kLoraThreads];
+struct LoraShrink {
+    static constexpr int kKWarps = kLoraWarps / MW, kRanks = 16 * MT * MW, kStride = 8 * NT + 1;
+    static constexpr int kBatch = 32 * kKWarps;  // columns from a warp's block to its next
+    struct Shared {
+        float parts[kKWarps][kRanks * kStride];
+        float4 sums[MT * NT][kLoraThreads];
+    };
     struct Batch {
         LoraEight<W> w[2 * MT];
         LoraEight<float> x[NT];
     };
-    grid_dependency_wait();  // the plan comes from the kernel before
-    allow_dependent_launch();
-    lora_tiles(tiles, p, blockIdx.x == 0);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = 4 * (lane & 3), t8 = 2 * t4;
-    const int chunks = (p.max_rank + kRanks - 1) / kRanks, per_tile = p.splits * chunks;
-    for (int64_t item = blockIdx.x; item < static_cast<int64_t>(tiles.count) * per_tile; item += gridDim.x) {
-        lora_open(tiles, p, static_cast<int>(item / per_tile));
-        const int part = static_cast<int>(item % per_tile), split = part / chunks, r0 = part % chunks * kRanks;
-        const int a = tiles.adapter, n = tiles.n, rank = lora_rank(p, a);
-        if (r0 >= rank) continue;
+
+    // Ranks r0 .. of adapter a (of its `rank`) and the columns of units first .. u1 of 16; the warps' sums stand in
+    // s.parts when it returns, for sum().
+    static __device__ __forceinline__ void run(const LoraArgs &p, Shared &s, const int (&tokens)[8 * NT], int a, int rank,
+                                               int r0, int first, int u1) {
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = 4 * (lane & 3), t8 = 2 * t4;
         const int kw = warp / MW, rw = r0 + 16 * MT * (warp % MW) + g;  // the lane's first rank
-        const int u0 = split * p.units + 2 * kw, u1 = min((split + 1) * p.units, (p.cols + 15) / 16);
+        const int u0 = first + 2 * kw;
         const W *w[2 * MT];
         const float *x[NT];
 #pragma unroll
@@ -347,7 +344,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(LoraArgs p
             w[i] = static_cast<const W *>(p.a) + (static_cast<int64_t>(a) * p.max_rank + r) * p.cols + 16 * u0 + t8;
         }
 #pragma unroll
-        for (int j = 0; j < NT; ++j) x[j] = p.x + tiles.tokens[8 * j + g] * p.x_stride + 16 * u0 + t8;
+        for (int j = 0; j < NT; ++j) x[j] = p.x + tokens[8 * j + g] * p.x_stride + 16 * u0 + t8;
         float acc[MT][NT][4] = {};
         const auto load = [&](Batch &t, int left) {  // left: columns from the lane's first to the end of the split
 #pragma unroll
@@ -377,7 +374,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(LoraArgs p
             for (int i = 0; i < MT; ++i) {
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
-                    float4 &sum = sums[i * NT + j][tid];
+                    float4 &sum = s.sums[i * NT + j][threadIdx.x];
                     float4 v = begun ? sum : make_float4(0.f, 0.f, 0.f, 0.f);
                     v.x += acc[i][j][0], v.y += acc[i][j][1], v.z += acc[i][j][2], v.w += acc[i][j][3];
                     sum = v;
@@ -405,7 +402,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(LoraArgs p
             for (int i = 0; i < MT; ++i) {
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
-                    const float4 v = sums[i * NT + j][tid];
+                    const float4 v = s.sums[i * NT + j][threadIdx.x];
                     acc[i][j][0] += v.x, acc[i][j][1] += v.y, acc[i][j][2] += v.z, acc[i][j][3] += v.w;
                 }
             }
@@ -415,54 +412,85 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(LoraArgs p
         for (int i = 0; i < MT; ++i) {
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-                float *at = parts[kw] + (rw - r0 + 16 * i) * kStride + 8 * j + t4 / 2;
+                float *at = s.parts[kw] + (rw - r0 + 16 * i) * kStride + 8 * j + t4 / 2;
                 at[0] = acc[i][j][0], at[1] = acc[i][j][1];
                 at[8 * kStride] = acc[i][j][2], at[8 * kStride + 1] = acc[i][j][3];
             }
         }
         __syncthreads();
-        const int ranks = min(kRanks, rank - r0);
-        for (int i = tid; i < n * kRanks; i += kLoraThreads) {
-            const int tok = i / kRanks, r = i % kRanks;
-            if (r >= ranks) continue;
-            float sum = 0.0f;
+    }
+
+    static __device__ __forceinline__ float sum(const Shared &s, int r, int tok) {
+        float v = 0.0f;
 #pragma unroll
-            for (int v = 0; v < kKWarps; ++v) sum += parts[v][r * kStride + tok];
-            p.h[(static_cast<int64_t>(split) * p.tokens + tiles.tokens[tok]) * p.max_rank + r0 + r] = sum;
+        for (int k = 0; k < kKWarps; ++k) v += s.parts[k][r * kStride + tok];
+        return v;
+    }
+};
+
+// h[split][token][r] = A[r][the split's columns] . x[token][the split's columns], item
+// after item (a tile, a split, a run of ranks).
+template <class W, int MT, int MW, int NT, bool VEC>
+__global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(LoraArgs p) {
+    using Shrink = LoraShrink<W, MT, MW, NT, VEC>;
+    constexpr int kRanks = Shrink::kRanks;
+    __shared__ LoraTiles<8 * NT> tiles;
+    __shared__ typename Shrink::Shared shared;
+    grid_dependency_wait();  // the plan comes from the kernel before
+    allow_dependent_launch();
+    lora_tiles(tiles, p, blockIdx.x == 0);
+    const int chunks = (p.max_rank + kRanks - 1) / kRanks, per_tile = p.splits * chunks;
+    for (int64_t item = blockIdx.x; item < static_cast<int64_t>(tiles.count) * per_tile; item += gridDim.x) {
+        lora_open(tiles, p, static_cast<int>(item / per_tile));
+        const int part = static_cast<int>(item % per_tile), split = part / chunks, r0 = part % chunks * kRanks;
+        const int rank = lora_rank(p, tiles.adapter);
+        if (r0 >= rank) continue;
+        Shrink::run(p, shared, tiles.tokens, tiles.adapter, rank, r0, split * p.units,
+                    min((split + 1) * p.units, (p.cols + 15) / 16));
+        for (int i = threadIdx.x; i < tiles.n * kRanks; i += kLoraThreads) {
+            const int tok = i / kRanks, r = i % kRanks;
+            if (r0 + r < rank)
+                p.h[(static_cast<int64_t>(split) * p.tokens + tiles.tokens[tok]) * p.max_rank + r0 + r] =
+                    Shrink::sum(shared, r, tok);
         }
     }
 }
 
-// y[token][row] += s * B[row] . h[token] for tiles of 8 NT tokens.  A CTA's share is
-// a run of the steps of all tiles (a step: 32 RG rows a warp).  Row 4 g + i of
-// 32 stands at place g of half i of two m16 tiles, so that a lane ends up with
+// The floats from one token's h to the next's in shared memory: 16 or 4 mod 32 banks, so that the quarters of a
+// warp's 16-byte reads do not meet.
+template <int KU>
+__host__ __device__ constexpr int lora_pitch(int rank) {
+    const int chunks = (rank + 16 * KU - 1) / (16 * KU);
+    return KU == 1 ? 16 * (chunks | 1) : 32 * chunks + 4;
+}
+
+// Element r of token tok's h, as hi + lo.
+template <int NT>
+__device__ __forceinline__ void lora_put(float *hs, int pitch, int tok, int r, float h) {
+    const uint32_t hi = lora_tf32(h);
+    hs[tok * pitch + r] = __uint_as_float(hi);
+    hs[(8 * NT + tok) * pitch + r] = __uint_as_float(lora_tf32(h - __uint_as_float(hi)));
+}
+
+// y[token][row] += s * B[row] . h[token] for a tile of 8 NT tokens, by one warp:
+// `steps` times 32 RG rows, from row_first, row_next apart.  Row 4 g + i of 32
+// stands at place g of half i of two m16 tiles, so that a lane ends up with
 // four neighbouring rows of two tokens: one float4 of y each.  Ranks come 16 KU at a
 // time.  With VEC lanes whose rows are behind the last read the last ones and write nothing.
+// prepare() puts h into hs (lora_put, zero from the rank to the end of its chunk) and
+// synchronises; the first weights are on their way meanwhile.
 template <class W, int NT, int RG, int KU, bool VEC>
-__global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(LoraArgs p) {
-    extern __shared__ __align__(16) float hs[];  // [2][8 NT][pitch]: hi, lo
-    __shared__ LoraTiles<8 * NT> tiles;
-    constexpr int kSpan = kLoraRows * RG, kNext = kLoraWarps * kSpan;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = 4 * (lane & 3);
-    lora_tiles(tiles, p, false);
-    bool waited = false;
-    const int per_tile = (p.rows + kNext - 1) / kNext;
-    const int64_t all = static_cast<int64_t>(tiles.count) * per_tile;
-    int64_t at = all * blockIdx.x / gridDim.x;
-    const int64_t end = all * (blockIdx.x + 1) / gridDim.x;
-    while (at < end) {
-        lora_open(tiles, p, static_cast<int>(at / per_tile));
-        const int first = static_cast<int>(at % per_tile);
-        const int steps = static_cast<int>(min(end - at, static_cast<int64_t>(per_tile - first)));
-        at += steps;
-        const int a = tiles.adapter, n = tiles.n, rank = lora_rank(p, a);
-        constexpr int kChunk = 16 * KU;
+struct LoraExpand {
+    static constexpr int kSpan = kLoraRows * RG, kChunk = 16 * KU;
+
+    template <class F>
+    static __device__ __forceinline__ void run(const LoraArgs &p, const float *hs, const int (&tokens)[8 * NT], int n, int a,
+                                               int rank, int row_first, int row_next, int steps, const F &prepare) {
+        const int t4 = 4 * (threadIdx.x & 3);
         const int chunks = (rank + kChunk - 1) / kChunk, lane_r = KU * t4;  // a lane has 4 KU neighbouring ranks of a chunk
-        if (rank == 0) continue;
-        // 16 or 4 mod 32 banks: the quarters of a warp's 16-byte reads do not meet
-        const int pitch = KU == 1 ? 16 * (chunks | 1) : kChunk * chunks + 4;
+        const int lane = threadIdx.x & 31, g = lane >> 2, pitch = lora_pitch<KU>(rank);
         const float scale = p.scales[a];
-        float *ls = hs + 8 * NT * pitch;
+        const float *ls = hs + 8 * NT * pitch;
         const W *b = static_cast<const W *>(p.b) + static_cast<int64_t>(a) * p.rows * p.max_rank + lane_r;
         float *y[NT][2];  // the lane's tokens' rows
         bool mine[NT][2];
@@ -472,7 +500,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(LoraArgs p
             for (int e = 0; e < 2; ++e) {
                 const int tok = 8 * j + t4 / 2 + e;
                 mine[j][e] = tok < n;
-                y[j][e] = p.y + tiles.tokens[tok] * p.y_stride;
+                y[j][e] = p.y + tokens[tok] * p.y_stride;
             }
         }
         struct Rows {
@@ -518,38 +546,17 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(LoraArgs p
         };
         // A turn: a chunk of ranks of a step's rows.  The weights of two turns are on their way while a third's are
         // multiplied; the three places take turns by name, since a copy from one to the next would wait for it.
-        int row = (first * kLoraWarps + warp) * kSpan + 4 * g, chunk = 0;
+        int row = row_first + 4 * g, chunk = 0;
         int fetch_row = row, fetch_chunk = 0, fetches = steps * chunks;
         const auto fetch = [&](Weights &to) {
             if (--fetches < 0) return;
             load_w(to, fetch_row, fetch_chunk);
-            if (++fetch_chunk == chunks) fetch_chunk = 0, fetch_row += kNext;
+            if (++fetch_chunk == chunks) fetch_chunk = 0, fetch_row += row_next;
         };
         Weights one, two, three;
         fetch(one);
         fetch(two);
-        // h, its parts joined in order, as hi + lo; zero behind the rank
-        if (!waited) grid_dependency_wait();  // h comes from the kernel before
-        waited = true;
-        for (int i = tid; i < 8 * NT * kChunk * chunks; i += kLoraThreads) {
-            const int tok = i / (kChunk * chunks), r = i - tok * kChunk * chunks;
-            float sum = 0.0f;
-            if (tok < n && r < rank) {
-                const float *h = p.h + static_cast<int64_t>(tiles.tokens[tok]) * p.max_rank + r;
-                const int64_t on = static_cast<int64_t>(p.tokens) * p.max_rank;
-                for (int s = 0; s < p.splits; s += 8) {  // eight in flight
-                    float part[8];
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) part[k] = s + k < p.splits ? h[(s + k) * on] : 0.0f;
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) sum += part[k];
-                }
-            }
-            const uint32_t hi = lora_tf32(sum);
-            hs[tok * pitch + r] = __uint_as_float(hi);
-            ls[tok * pitch + r] = __uint_as_float(lora_tf32(sum - __uint_as_float(hi)));
-        }
-        __syncthreads();
+        prepare();
         LoraRaw<W> last_mask[KU];
 #pragma unroll
         for (int k = 0; k < KU; ++k) last_mask[k] = lora_mask<W>(rank - kChunk * (chunks - 1) - lane_r - 4 * k);
@@ -609,7 +616,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(LoraArgs p
                     }
                 }
             }
-            row += kNext;
+            row += row_next;
         };
         for (int left = steps * chunks; left > 0; left -= 3) {
             turn(one, three);
@@ -617,8 +624,117 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(LoraArgs p
             if (left > 2) turn(three, two);
         }
     }
+};
+
+// The tiles' steps in one row, a run of them a CTA; h from the workspace, its parts joined in order.
+template <class W, int NT, int RG, int KU, bool VEC>
+__global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(LoraArgs p) {
+    using Expand = LoraExpand<W, NT, RG, KU, VEC>;
+    extern __shared__ __align__(16) float hs[];  // [2][8 NT][pitch]: hi, lo
+    __shared__ LoraTiles<8 * NT> tiles;
+    constexpr int kNext = kLoraWarps * Expand::kSpan;
+    const int tid = threadIdx.x, warp = tid >> 5;
+    lora_tiles(tiles, p, false);
+    bool waited = false;
+    const int per_tile = (p.rows + kNext - 1) / kNext;
+    const int64_t all = static_cast<int64_t>(tiles.count) * per_tile, end = all * (blockIdx.x + 1) / gridDim.x;
+    int64_t at = all * blockIdx.x / gridDim.x;
+    while (at < end) {
+        lora_open(tiles, p, static_cast<int>(at / per_tile));
+        const int first = static_cast<int>(at % per_tile);
+        const int steps = static_cast<int>(min(end - at, static_cast<int64_t>(per_tile - first)));
+        at += steps;
+        const int rank = lora_rank(p, tiles.adapter);
+        if (rank == 0) continue;
+        Expand::run(p, hs, tiles.tokens, tiles.n, tiles.adapter, rank, (first * kLoraWarps + warp) * Expand::kSpan, kNext,
+                    steps, [&]() {
+            if (!waited) grid_dependency_wait();  // h comes from the kernel before
+            waited = true;
+            const int width = (rank + Expand::kChunk - 1) / Expand::kChunk * Expand::kChunk;
+            for (int i = tid; i < 8 * NT * width; i += kLoraThreads) {
+                const int tok = i / width, r = i - tok * width;
+                float sum = 0.0f;
+                if (tok < tiles.n && r < rank) {
+                    const float *h = p.h + static_cast<int64_t>(tiles.tokens[tok]) * p.max_rank + r;
+                    const int64_t on = static_cast<int64_t>(p.tokens) * p.max_rank;
+                    for (int s = 0; s < p.splits; s += 8) {  // eight in flight
+                        float part[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) part[k] = s + k < p.splits ? h[(s + k) * on] : 0.0f;
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) sum += part[k];
+                    }
+                }
+                lora_put<NT>(hs, lora_pitch<KU>(rank), tok, r, sum);
+            }
+            __syncthreads();
+        });
+    }
     // A CTA with nothing to do must not end before the kernel before: what comes next waits for this one only.
     if (!waited) grid_dependency_wait();
+}
+
+// Few tiles of small adapters in one launch: a cluster per tile.  Each CTA takes a share of the columns, the
+// cluster's CTAs read one another's sums, and each takes a share of the rows.  For adapters of up to kLoraSmall bytes
+// whose clusters have an SM a CTA at once; in CUDA graphs, this against the two kernels: 1 token, 576 x 6144 of rank 8
+// 5.5 against 6.1 us, 512 x 512 of rank 64 5.8 against 7.3; 16 tokens of 16 adapters, 2048 x 6144 of rank 16 7.4
+// against 8.3.  Beyond: one of 4096 x 4096 of rank 64 (1 MB) 8.5 against 7.3, 36 adapters of 256 x 256 8.9 against 5.6.
+constexpr int kLoraCluster = 8;
+constexpr int64_t kLoraSmall = 512 << 10;
+
+__device__ __forceinline__ float cluster_load(const float *at, uint32_t rank) {  // this CTA's `at` in CTA `rank`
+    uint32_t remote;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_addr(at)), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
+    return v;
+}
+
+template <class W, int MT, int MW, int RG, int KU, bool VEC>
+__global__ void __launch_bounds__(kLoraThreads, 2) lora_cluster_kernel(LoraArgs p) {
+    using Shrink = LoraShrink<W, MT, MW, 1, VEC>;
+    using Expand = LoraExpand<W, 1, RG, KU, VEC>;
+    extern __shared__ __align__(16) float hs[];  // [2][8][pitch]: hi, lo; then this CTA's sums [8][max_rank]
+    __shared__ LoraTiles<8> tiles;
+    __shared__ typename Shrink::Shared shared;
+    const int tid = threadIdx.x, part = blockIdx.x % kLoraCluster, tile = blockIdx.x / kLoraCluster;
+    lora_tiles(tiles, p, blockIdx.x == 0);
+    if (tile >= tiles.count) return;  // the whole cluster
+    lora_open(tiles, p, tile);
+    const int rank = lora_rank(p, tiles.adapter), n = tiles.n, pitch = lora_pitch<KU>(rank);
+    if (rank == 0) return;  // the whole cluster
+    float *mine = hs + 16 * lora_pitch<KU>(p.max_rank);
+    const int units = (p.cols + 15) / 16, share = 2 * ((units + 2 * kLoraCluster - 1) / (2 * kLoraCluster));
+    for (int r0 = 0; r0 < rank; r0 += Shrink::kRanks) {
+        if (r0) __syncthreads();  // the ranks before are read
+        Shrink::run(p, shared, tiles.tokens, tiles.adapter, rank, r0, part * share, min((part + 1) * share, units));
+        for (int i = tid; i < n * Shrink::kRanks; i += kLoraThreads) {
+            const int tok = i / Shrink::kRanks, r = i % Shrink::kRanks;
+            if (r0 + r < rank) mine[tok * p.max_rank + r0 + r] = Shrink::sum(shared, r, tok);
+        }
+    }
+    cluster_arrive();
+    const int row_first = (part * kLoraWarps + (tid >> 5)) * Expand::kSpan, row_next = kLoraCluster * kLoraWarps * Expand::kSpan;
+    const int steps = row_first < p.rows ? (p.rows - row_first + row_next - 1) / row_next : 0;
+    Expand::run(p, hs, tiles.tokens, n, tiles.adapter, rank, row_first, row_next, steps, [&]() {
+        cluster_wait();
+        const int width = (rank + Expand::kChunk - 1) / Expand::kChunk * Expand::kChunk;
+        for (int i = tid; i < 8 * width; i += kLoraThreads) {
+            const int tok = i / width, r = i - tok * width;
+            float sum = 0.0f;
+            if (tok < n && r < rank) {
+                float v[kLoraCluster];
+#pragma unroll
+                for (int c = 0; c < kLoraCluster; ++c) v[c] = cluster_load(mine + tok * p.max_rank + r, c);
+#pragma unroll
+                for (int c = 0; c < kLoraCluster; ++c) sum += v[c];
+            }
+            lora_put<1>(hs, pitch, tok, r, sum);
+        }
+        cluster_arrive();
+        __syncthreads();
+    });
+    cluster_wait();  // this CTA's sums are read
 }
 
 constexpr int lora_ceil(int64_t n, int64_t of) { return static_cast<int>((n + of - 1) / of); }
@@ -674,19 +790,45 @@ int32_t lora_shrink(const LoraArgs &p, dim3 grid, bool vec, cudaStream_t stream)
 
 template <class W, int NT, int RG, int KU>
 int32_t lora_expand(const LoraArgs &p, dim3 grid, bool vec, cudaStream_t stream) {
-    const int chunks = lora_ceil(p.max_rank, 16 * KU), pitch = KU == 1 ? 16 * (chunks | 1) : 32 * chunks + 4;
-    const size_t smem = sizeof(float) * 2 * 8 * NT * pitch;
+    const size_t smem = sizeof(float) * 2 * 8 * NT * lora_pitch<KU>(p.max_rank);
     const auto kernel = vec ? lora_expand_kernel<W, NT, RG, KU, true> : lora_expand_kernel<W, NT, RG, KU, false>;
     if (const int32_t rc = allow_dynamic_smem(kernel, smem, "lora_expand smem")) return rc;
     return lora_start(kernel, grid, smem, p, true, stream, "lora_expand_kernel");
 }
 
+template <class W, int MT, int MW, int RG, int KU>
+int32_t lora_cluster(const LoraArgs &p, int tiles, bool vec, cudaStream_t stream) {
+    const auto kernel = vec ? lora_cluster_kernel<W, MT, MW, RG, KU, true> : lora_cluster_kernel<W, MT, MW, RG, KU, false>;
+    const size_t smem = sizeof(float) * (16 * lora_pitch<KU>(p.max_rank) + 8 * p.max_rank);
+    if (const int32_t rc = allow_dynamic_smem(kernel, smem, "lora_cluster smem")) return rc;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = kLoraCluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(tiles * kLoraCluster);
+    cfg.blockDim = dim3(kLoraThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    GLMVX_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
+    return launch_status("lora_cluster_kernel");
+}
+
 template <class W, int NT>
 int32_t lora_launch(LoraArgs &p, bool vec_a, bool vec_b, cudaStream_t stream) {
     const int sms = sm_count();
-    // CTAs along the tokens: every token may lead a tile, or the plan's most.
-    const int tiles = p.tiles ? static_cast<int>(std::min<int64_t>(p.tokens, p.tokens / (8 * NT) + int64_t{p.adapters}))
-                              : p.tokens;
+    // There are at most this many tiles: each but an adapter's last one is full.
+    const int tiles = static_cast<int>(std::min<int64_t>(p.tokens, p.tokens / (8 * NT) + int64_t{p.adapters}));
+    const int64_t weights = static_cast<int64_t>(p.rows + p.cols) * p.max_rank * static_cast<int64_t>(sizeof(W));
+    if (NT == 1 && tiles * kLoraCluster <= sms && weights <= kLoraSmall) {
+        const bool vec = vec_a && vec_b;
+        constexpr int kTwo = sizeof(W) == 4 ? 1 : 2;
+        if (p.max_rank <= 16) return lora_cluster<W, 1, 1, kTwo, 1>(p, tiles, vec, stream);
+        if (p.max_rank <= 32) return lora_cluster<W, 2, 1, 1, kTwo>(p, tiles, vec, stream);
+        return lora_cluster<W, 2, 2, 1, kTwo>(p, tiles, vec, stream);
+    }
     if (p.tiles) {
         lora_plan_kernel<<<1, kLoraPlanThreads, 0, stream>>>(p, 8 * NT);
         if (const int32_t rc = launch_status("lora_plan_kernel")) return rc;

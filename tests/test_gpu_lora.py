@@ -245,6 +245,34 @@ def test_ranks_and_widths_on_both_sides_of_the_tiles(gpu_backend, kind, max_rank
              ranks=[max_rank, max(1, max_rank // 2 + 1), 1], seed=tokens + cols).check(gpu_backend)
 
 
+@pytest.mark.parametrize('kind', [0, 1, 30])
+@pytest.mark.parametrize('max_rank,cols,rows', [(1, 31, 5), (16, 512, 256), (19, 515, 130), (33, 1000, 132), (64, 64, 1028),
+                                                (256, 264, 36)])
+def test_few_tokens_in_one_launch_and_in_two(gpu_backend, kind, max_rank, cols, rows):
+    """The number of tiles there may be (tokens, or an eighth of them and one an adapter) decides: from 19 on, two
+    launches; both with ranks that differ and adapters that several tiles share."""
+    for tokens, adapters in ((18, 40), (19, 40), (64, 3), (64, 90)):
+        rng = np.random.default_rng(tokens + adapters)
+        ids = np.where(rng.random(tokens) < 0.5, rng.integers(-1, 3, tokens), rng.integers(0, adapters, tokens))
+        Case(tokens, rows, cols, adapters, max_rank, kind, ids=ids, seed=tokens + cols).check(gpu_backend)
+
+
+@pytest.mark.parametrize('tokens,adapters,max_rank,cols,rows', [(1, 1, 16, 8192, 8192), (1, 1, 16, 8192, 8196),
+                                                                (9, 2, 64, 4096, 64), (9, 2, 64, 4088, 8)])
+def test_adapters_around_the_size_for_one_launch(gpu_backend, tokens, adapters, max_rank, cols, rows):
+    Case(tokens, rows, cols, adapters, max_rank, 30, ids=np.arange(tokens) % adapters, ranks=[max_rank] * adapters,
+         seed=rows).check(gpu_backend)
+
+
+@pytest.mark.parametrize('kind', [0, 30])
+def test_a_token_of_two_launches_does_not_depend_on_the_others(gpu_backend, kind):
+    case = Case(40, 96, 320, 50, 16, kind, ids=np.arange(40) % 7, ranks=[16, 7, 1, 16, 12] * 10, seed=4)
+    out = case.run(gpu_backend)
+    case.ids[case.ids != 3] = -1
+    alone = case.run(gpu_backend)
+    assert alone[3::7].tobytes() == out[3::7].tobytes()
+
+
 def test_many_adapters_and_many_tokens(gpu_backend):
     """More adapters than the plan counts in shared memory, more tokens than its threads keep."""
     Case(200, 8, 16, 5000, 2, 1, seed=1).check(gpu_backend)
