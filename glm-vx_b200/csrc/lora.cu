@@ -37,9 +37,10 @@ constexpr int kLoraMaxSplits = 32;
 constexpr int kLoraRankChunk = 64;   // ranks a shrink CTA takes
 constexpr int kLoraRows = 32;        // rows of B a warp takes at once
 
-// A tile of the plan: n tokens of one adapter, order[start ..].
+// A tile of the plan: n tokens of one adapter (the places behind them hold anything).
+constexpr int kLoraTile = 16;
 struct LoraTile {
-    int adapter, start, n, pad;
+    int adapter, n, rank, pad, tokens[kLoraTile];
 };
 
 struct LoraArgs {
@@ -51,7 +52,7 @@ struct LoraArgs {
     const float *scales;
     float *h;         // [splits][tokens][max_rank]
     LoraTile *tiles;  // the plan (NULL: CTAs scan the ids)
-    int *order, *counts, *places, *ntiles;
+    int *counts, *places, *ntiles;
     int64_t y_stride, x_stride;
     int tokens, rows, cols, adapters, max_rank, splits, units;
     int *err;
@@ -189,9 +190,9 @@ __device__ __forceinline__ void lora_unit(float (&c)[4], const float4 &top, cons
 template <int TILE>
 struct LoraTiles {
     int count;
-    int tokens[TILE], adapter, n;  // of the tile last opened
+    int tokens[TILE], adapter, n, rank;  // of the tile last opened
     int ids[kLoraScan], leads[kLoraScan / 32];
-    int tile_adapter[kLoraScan], tile_n[kLoraScan], tile_tokens[kLoraScan][TILE];
+    int tile_adapter[kLoraScan], tile_n[kLoraScan], tile_rank[kLoraScan], tile_tokens[kLoraScan][TILE];
 };
 
 template <int TILE>
@@ -202,7 +203,7 @@ __device__ __forceinline__ void lora_tiles(LoraTiles<TILE> &s, const LoraArgs &p
         __syncthreads();
         return;
     }
-    int a = -1;
+    int a = -1, rank = 0;
     if (tid < kLoraScan) {
         a = tid < p.tokens ? p.ids[tid] : -1;
         if (a >= p.adapters) {
@@ -210,6 +211,7 @@ __device__ __forceinline__ void lora_tiles(LoraTiles<TILE> &s, const LoraArgs &p
             a = -1;
         }
         s.ids[tid] = a;
+        rank = __ldg(p.ranks + max(a, 0));  // on its way while the tiles are found
     }
     __syncthreads();
     uint64_t same = 0;  // the tokens of this one's adapter
@@ -229,6 +231,7 @@ __device__ __forceinline__ void lora_tiles(LoraTiles<TILE> &s, const LoraArgs &p
         for (uint64_t left = same >> tid << tid; left && n < TILE; left &= left - 1) s.tile_tokens[k][n++] = __ffsll(left) - 1;
         s.tile_adapter[k] = a;
         s.tile_n[k] = n;
+        s.tile_rank[k] = min(max(rank, 0), p.max_rank);
     }
     if (tid == 0) {
         int all = 0;
@@ -238,29 +241,38 @@ __device__ __forceinline__ void lora_tiles(LoraTiles<TILE> &s, const LoraArgs &p
     __syncthreads();
 }
 
-// Opens tile k: its adapter, its tokens (of those it lacks, its first).
+// Opens tile k: its adapter and rank, its tokens (of those it lacks, its first).
 template <int TILE>
 __device__ __forceinline__ void lora_open(LoraTiles<TILE> &s, const LoraArgs &p, int k) {
-    __syncthreads();  // the tile before is done with
     const int tid = threadIdx.x;
+    int v = 0;
+    if (p.tiles && tid < 32) {  // on its way while the CTA meets
+        static_assert(sizeof(LoraTile) == 4 * (4 + kLoraTile) && kLoraTile <= 28);
+        if (tid < 4 + kLoraTile) v = reinterpret_cast<const int *>(p.tiles + k)[tid];
+    }
+    __syncthreads();  // the tile before is done with
     if (p.tiles) {
-        const LoraTile tile = p.tiles[k];
-        if (tid < TILE) s.tokens[tid] = p.order[tile.start + (tid < tile.n ? tid : 0)];
-        if (tid == 0) s.adapter = tile.adapter, s.n = tile.n;
+        if (tid < 32) {
+            const int n = __shfl_sync(0xffffffffu, v, 1), first = __shfl_sync(0xffffffffu, v, 4);
+            if (tid >= 4 && tid < 4 + TILE) s.tokens[tid - 4] = tid - 4 < n ? v : first;
+            if (tid == 0) s.adapter = v;
+            if (tid == 1) s.n = v;
+            if (tid == 2) s.rank = v;
+        }
     } else {
         if (tid < TILE) s.tokens[tid] = s.tile_tokens[k][tid < s.tile_n[k] ? tid : 0];
-        if (tid == 0) s.adapter = s.tile_adapter[k], s.n = s.tile_n[k];
+        if (tid == 0) s.adapter = s.tile_adapter[k], s.n = s.tile_n[k], s.rank = s.tile_rank[k];
     }
     __syncthreads();
 }
 
-// Tiles of up to `tile` tokens of one adapter: one CTA counts the adapters'
-// tokens (in shared memory when the adapters fit), gives each adapter its place
-// in the order, and lists the tiles.  The order within an adapter is that of
-// the atomics, which no result depends on.
+// Tiles of up to kLoraTile tokens of one adapter: one CTA counts the adapters' tokens
+// (in shared memory when the adapters fit), gives each adapter its tiles, and each
+// token its place in them.  The order within an adapter is that of the atomics,
+// which no result depends on.
 constexpr int kLoraPlanThreads = 1024, kLoraPlanOwn = 4, kLoraPlanCounts = 4096;
-__global__ void __launch_bounds__(kLoraPlanThreads) lora_plan_kernel(LoraArgs p, int tile) {
-    __shared__ int warp_tokens[32], warp_tiles[32], near_counts[kLoraPlanCounts];
+__global__ void __launch_bounds__(kLoraPlanThreads) lora_plan_kernel(LoraArgs p) {
+    __shared__ int warp_tiles[32], near_counts[kLoraPlanCounts];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     allow_dependent_launch();
     int *counts = p.adapters <= kLoraPlanCounts ? near_counts : p.counts;
@@ -268,47 +280,55 @@ __global__ void __launch_bounds__(kLoraPlanThreads) lora_plan_kernel(LoraArgs p,
     int own[kLoraPlanOwn], place[kLoraPlanOwn];  // the thread's first tokens
 #pragma unroll
     for (int k = 0; k < kLoraPlanOwn; ++k) {
-        const int t = tid + k * kLoraPlanThreads, a = t < p.tokens ? p.ids[t] : -1;
-        if (a >= p.adapters) report_device_error(p.err, kDevErrBadIndex);
-        own[k] = a < p.adapters ? a : -1;
+        const int t = tid + k * kLoraPlanThreads;
+        own[k] = t < p.tokens ? p.ids[t] : -1;
     }
+    int rank = tid < p.adapters ? lora_rank(p, tid) : 0;
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kLoraPlanOwn; ++k) place[k] = own[k] >= 0 ? atomicAdd(counts + own[k], 1) : 0;
+    for (int k = 0; k < kLoraPlanOwn; ++k) {
+        if (own[k] >= p.adapters) {
+            report_device_error(p.err, kDevErrBadIndex);
+            own[k] = -1;
+        }
+        place[k] = own[k] >= 0 ? atomicAdd(counts + own[k], 1) : 0;
+    }
     for (int t = tid + kLoraPlanOwn * kLoraPlanThreads; t < p.tokens; t += kLoraPlanThreads) {
         const int a = p.ids[t];
         if (a >= p.adapters) report_device_error(p.err, kDevErrBadIndex);
         p.places[t] = a >= 0 && a < p.adapters ? atomicAdd(counts + a, 1) : 0;
     }
     __syncthreads();
-    int token_base = 0, tile_base = 0;  // of the adapters before this round's
+    int base = 0;  // the tiles of the adapters before this round's
     for (int a0 = 0; a0 < p.adapters; a0 += kLoraPlanThreads) {
-        const int a = a0 + tid, n = a < p.adapters ? counts[a] : 0, nt = (n + tile - 1) / tile;
-        int sn = n, st = nt;
+        const int a = a0 + tid, n = a < p.adapters ? counts[a] : 0, nt = (n + kLoraTile - 1) / kLoraTile;
+        if (a0) rank = a < p.adapters ? lora_rank(p, a) : 0;
+        int sum = nt;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int un = __shfl_up_sync(0xffffffffu, sn, o), ut = __shfl_up_sync(0xffffffffu, st, o);
-            if (lane >= o) sn += un, st += ut;
+            const int up = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += up;
         }
-        if (lane == 31) warp_tokens[warp] = sn, warp_tiles[warp] = st;
+        if (lane == 31) warp_tiles[warp] = sum;
         __syncthreads();
-        int start = token_base + sn - n, first = tile_base + st - nt;
-        for (int w = 0; w < kLoraPlanThreads / 32; ++w) {
-            if (w < warp) start += warp_tokens[w], first += warp_tiles[w];
-            token_base += warp_tokens[w], tile_base += warp_tiles[w];
-        }
-        if (a < p.adapters) counts[a] = start;
-        for (int i = 0; i < nt; ++i) p.tiles[first + i] = {a, start + i * tile, min(tile, n - i * tile), 0};
+        int first = base + sum - nt, all = warp_tiles[lane];
+        const int before = __reduce_add_sync(0xffffffffu, lane < warp ? all : 0);
+        first += before;
+        base += __reduce_add_sync(0xffffffffu, all);
+        if (a < p.adapters) counts[a] = first;
+        for (int i = 0; i < nt; ++i)
+            *reinterpret_cast<int4 *>(p.tiles + first + i) = make_int4(a, min(kLoraTile, n - i * kLoraTile), rank, 0);
         __syncthreads();
     }
+    const auto put = [&](int a, int at, int t) { p.tiles[counts[a] + at / kLoraTile].tokens[at % kLoraTile] = t; };
 #pragma unroll
     for (int k = 0; k < kLoraPlanOwn; ++k)
-        if (own[k] >= 0) p.order[counts[own[k]] + place[k]] = tid + k * kLoraPlanThreads;
+        if (own[k] >= 0) put(own[k], place[k], tid + k * kLoraPlanThreads);
     for (int t = tid + kLoraPlanOwn * kLoraPlanThreads; t < p.tokens; t += kLoraPlanThreads) {
         const int a = p.ids[t];
-        if (a >= 0 && a < p.adapters) p.order[counts[a] + p.places[t]] = t;
+        if (a >= 0 && a < p.adapters) put(a, p.places[t], t);
     }
-    if (tid == 0) *p.ntiles = tile_base;
+    if (tid == 0) *p.ntiles = base;
 }
 
 // A . x for a tile of 8 NT tokens, 16 MT MW ranks and a range of columns, by one
@@ -443,7 +463,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(LoraArgs p
     for (int64_t item = blockIdx.x; item < static_cast<int64_t>(tiles.count) * per_tile; item += gridDim.x) {
         lora_open(tiles, p, static_cast<int>(item / per_tile));
         const int part = static_cast<int>(item % per_tile), split = part / chunks, r0 = part % chunks * kRanks;
-        const int rank = lora_rank(p, tiles.adapter);
+        const int rank = tiles.rank;
         if (r0 >= rank) continue;
         Shrink::run(p, shared, tiles.tokens, tiles.adapter, rank, r0, split * p.units,
                     min((split + 1) * p.units, (p.cols + 15) / 16));
@@ -644,7 +664,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(LoraArgs p
         const int first = static_cast<int>(at % per_tile);
         const int steps = static_cast<int>(min(end - at, static_cast<int64_t>(per_tile - first)));
         at += steps;
-        const int rank = lora_rank(p, tiles.adapter);
+        const int rank = tiles.rank;
         if (rank == 0) continue;
         Expand::run(p, hs, tiles.tokens, tiles.n, tiles.adapter, rank, (first * kLoraWarps + warp) * Expand::kSpan, kNext,
                     steps, [&]() {
@@ -701,7 +721,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_cluster_kernel(LoraArgs 
     lora_tiles(tiles, p, blockIdx.x == 0);
     if (tile >= tiles.count) return;  // the whole cluster
     lora_open(tiles, p, tile);
-    const int rank = lora_rank(p, tiles.adapter), n = tiles.n, pitch = lora_pitch<KU>(rank);
+    const int rank = tiles.rank, n = tiles.n, pitch = lora_pitch<KU>(rank);
     if (rank == 0) return;  // the whole cluster
     float *mine = hs + 16 * lora_pitch<KU>(p.max_rank);
     const int units = (p.cols + 15) / 16, share = 2 * ((units + 2 * kLoraCluster - 1) / (2 * kLoraCluster));
@@ -742,9 +762,12 @@ constexpr int lora_ceil(int64_t n, int64_t of) { return static_cast<int>((n + of
 // Parts that the columns are cut into, at most: enough CTAs for few tokens.
 int lora_max_splits(int tokens) { return std::clamp(lora_ceil(16384, tokens), 1, kLoraMaxSplits); }
 
-// The workspace: h, then (where there is a plan) the tiles, the order, the places, the counts.
+// Tiles of `size` tokens there may be: each but an adapter's last one is full.
+int64_t lora_most_tiles(int64_t tokens, int64_t adapters, int size) { return std::min(tokens, tokens / size + adapters); }
+
+// The workspace: h, then (where there is a plan) the tiles, the places, the counts.
 struct LoraLayout {
-    int64_t tiles, order, places, counts, ntiles, bytes;
+    int64_t tiles, places, counts, ntiles, bytes;
 };
 LoraLayout lora_layout(int64_t tokens, int64_t adapters, int64_t max_rank) {
     LoraLayout l{};
@@ -756,8 +779,7 @@ LoraLayout lora_layout(int64_t tokens, int64_t adapters, int64_t max_rank) {
     };
     take(4 * tokens * max_rank * lora_max_splits(static_cast<int>(tokens)));
     if (tokens > kLoraScan) {
-        l.tiles = take(sizeof(LoraTile) * tokens);
-        l.order = take(4 * tokens);
+        l.tiles = take(sizeof(LoraTile) * lora_most_tiles(tokens, adapters, kLoraTile));
         l.places = take(4 * tokens);
         l.counts = take(4 * adapters);
         l.ntiles = take(4);
@@ -819,8 +841,7 @@ int32_t lora_cluster(const LoraArgs &p, int tiles, bool vec, cudaStream_t stream
 template <class W, int NT>
 int32_t lora_launch(LoraArgs &p, bool vec_a, bool vec_b, cudaStream_t stream) {
     const int sms = sm_count();
-    // There are at most this many tiles: each but an adapter's last one is full.
-    const int tiles = static_cast<int>(std::min<int64_t>(p.tokens, p.tokens / (8 * NT) + int64_t{p.adapters}));
+    const int tiles = static_cast<int>(lora_most_tiles(p.tokens, p.adapters, 8 * NT));
     const int64_t weights = static_cast<int64_t>(p.rows + p.cols) * p.max_rank * static_cast<int64_t>(sizeof(W));
     if (NT == 1 && tiles * kLoraCluster <= sms && weights <= kLoraSmall) {
         const bool vec = vec_a && vec_b;
@@ -830,7 +851,8 @@ int32_t lora_launch(LoraArgs &p, bool vec_a, bool vec_b, cudaStream_t stream) {
         return lora_cluster<W, 2, 2, 1, kTwo>(p, tiles, vec, stream);
     }
     if (p.tiles) {
-        lora_plan_kernel<<<1, kLoraPlanThreads, 0, stream>>>(p, 8 * NT);
+        static_assert(NT == 1 || 8 * NT == kLoraTile);
+        lora_plan_kernel<<<1, kLoraPlanThreads, 0, stream>>>(p);
         if (const int32_t rc = launch_status("lora_plan_kernel")) return rc;
     }
     // Columns in as many parts as give two items an SM were every tile full, none shorter than four units a warp.
@@ -897,7 +919,6 @@ GLMVX_EXPORT int32_t glmvx_lora_add(float *y, int64_t y_stride, const float *x, 
     p.h = reinterpret_cast<float *>(ws);
     if (tokens > kLoraScan) {
         p.tiles = reinterpret_cast<LoraTile *>(ws + layout.tiles);
-        p.order = reinterpret_cast<int *>(ws + layout.order);
         p.places = reinterpret_cast<int *>(ws + layout.places);
         p.counts = reinterpret_cast<int *>(ws + layout.counts);
         p.ntiles = reinterpret_cast<int *>(ws + layout.ntiles);
