@@ -50,14 +50,15 @@ struct LoraArgs {
     const void *a, *b;
     const int32_t *ranks;
     const float *scales;
-    float *h;         // [splits][tokens][max_rank]
+    float *h;         // [splits][tokens][lora_h_pitch(max_rank)]
     LoraTile *tiles;  // the plan (NULL: CTAs scan the ids)
     int *counts, *places, *ntiles;
     int64_t y_stride, x_stride;
-    int tokens, rows, cols, adapters, max_rank, splits, units;
+    int tokens, rows, cols, adapters, max_rank, splits, units, team;
     int *err;
 };
 
+__host__ __device__ constexpr int lora_h_pitch(int max_rank) { return (max_rank + 3) & ~3; }
 __device__ __forceinline__ int lora_rank(const LoraArgs &p, int a) { return min(max(p.ranks[a], 0), p.max_rank); }
 
 // Four neighbouring values as they stand in memory; those from `n` on are 0
@@ -198,8 +199,8 @@ struct LoraTiles {
 template <int TILE>
 __device__ __forceinline__ void lora_tiles(LoraTiles<TILE> &s, const LoraArgs &p, bool report) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (p.tiles) {
-        if (tid == 0) s.count = *p.ntiles;
+    if (p.tiles) {  // read past L1: written by a kernel that may have run beside this one
+        if (tid == 0) s.count = __ldcg(p.ntiles);
         __syncthreads();
         return;
     }
@@ -248,7 +249,7 @@ __device__ __forceinline__ void lora_open(LoraTiles<TILE> &s, const LoraArgs &p,
     int v = 0;
     if (p.tiles && tid < 32) {  // on its way while the CTA meets
         static_assert(sizeof(LoraTile) == 4 * (4 + kLoraTile) && kLoraTile <= 28);
-        if (tid < 4 + kLoraTile) v = reinterpret_cast<const int *>(p.tiles + k)[tid];
+        if (tid < 4 + kLoraTile) v = __ldcg(reinterpret_cast<const int *>(p.tiles + k) + tid);
     }
     __syncthreads();  // the tile before is done with
     if (p.tiles) {
@@ -470,7 +471,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(LoraArgs p
         for (int i = threadIdx.x; i < tiles.n * kRanks; i += kLoraThreads) {
             const int tok = i / kRanks, r = i % kRanks;
             if (r0 + r < rank)
-                p.h[(static_cast<int64_t>(split) * p.tokens + tiles.tokens[tok]) * p.max_rank + r0 + r] =
+                p.h[(static_cast<int64_t>(split) * p.tokens + tiles.tokens[tok]) * lora_h_pitch(p.max_rank) + r0 + r] =
                     Shrink::sum(shared, r, tok);
         }
     }
@@ -490,6 +491,15 @@ __device__ __forceinline__ void lora_put(float *hs, int pitch, int tok, int r, f
     const uint32_t hi = lora_tf32(h);
     hs[tok * pitch + r] = __uint_as_float(hi);
     hs[(8 * NT + tok) * pitch + r] = __uint_as_float(lora_tf32(h - __uint_as_float(hi)));
+}
+
+// Elements r .. r + 3 of token tok's h.
+template <int NT>
+__device__ __forceinline__ void lora_put(float *hs, int pitch, int tok, int r, const float4 &h) {
+    uint32_t hi[4], lo[4];
+    lora_split(h, hi, lo);
+    *reinterpret_cast<uint4 *>(hs + tok * pitch + r) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    *reinterpret_cast<uint4 *>(hs + (8 * NT + tok) * pitch + r) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
 }
 
 // y[token][row] += s * B[row] . h[token] for a tile of 8 NT tokens, by one warp:
@@ -670,22 +680,38 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(LoraArgs p
                     steps, [&]() {
             if (!waited) grid_dependency_wait();  // h comes from the kernel before
             waited = true;
-            const int width = (rank + Expand::kChunk - 1) / Expand::kChunk * Expand::kChunk;
-            for (int i = tid; i < 8 * NT * width; i += kLoraThreads) {
-                const int tok = i / width, r = i - tok * width;
-                float sum = 0.0f;
+            // Each quad of ranks is summed by 2^team lanes, four parts in flight in each: the joining is bound by
+            // its instructions (of 32 parts, rank 64: a quad at once 33.4 us, single values, eight parts in flight,
+            // 37.8, sixteen 40.2, of a call of 1000 tokens).
+            const int quads = (rank + Expand::kChunk - 1) / Expand::kChunk * (Expand::kChunk / 4), items = 8 * NT * quads;
+            const int shift = p.team, team = 1 << shift, member = tid & (team - 1);
+            for (int i0 = 0; i0 < items; i0 += kLoraThreads >> shift) {
+                const int i = i0 + (tid >> shift), tok = i / quads, r = 4 * (i - tok * quads);
+                float4 sum{};
                 if (tok < tiles.n && r < rank) {
-                    const float *h = p.h + static_cast<int64_t>(tiles.tokens[tok]) * p.max_rank + r;
-                    const int64_t on = static_cast<int64_t>(p.tokens) * p.max_rank;
-                    for (int s = 0; s < p.splits; s += 8) {  // eight in flight
-                        float part[8];
+                    const int pitch = lora_h_pitch(p.max_rank);
+                    const float *h = p.h + static_cast<int64_t>(tiles.tokens[tok]) * pitch + r;
+                    const int64_t on = static_cast<int64_t>(p.tokens) * pitch << shift;
+                    h += member * (on >> shift);
+                    for (int s = member; s < p.splits; s += 4 * team, h += 4 * on) {
+                        float4 part[4];
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) part[k] = s + k < p.splits ? h[(s + k) * on] : 0.0f;
+                        for (int k = 0; k < 4; ++k)
+                            part[k] = s + k * team < p.splits ? *reinterpret_cast<const float4 *>(h + k * on)
+                                                              : float4{};
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) sum += part[k];
+                        for (int k = 0; k < 4; ++k)
+                            sum.x += part[k].x, sum.y += part[k].y, sum.z += part[k].z, sum.w += part[k].w;
                     }
                 }
-                lora_put<NT>(hs, lora_pitch<KU>(rank), tok, r, sum);
+                for (int o = 1; o < team; o *= 2) {
+                    sum.x += __shfl_xor_sync(0xffffffffu, sum.x, o), sum.y += __shfl_xor_sync(0xffffffffu, sum.y, o);
+                    sum.z += __shfl_xor_sync(0xffffffffu, sum.z, o), sum.w += __shfl_xor_sync(0xffffffffu, sum.w, o);
+                }
+                if (member == 0 && i < items) {
+                    sum.y = r + 1 < rank ? sum.y : 0.0f, sum.z = r + 2 < rank ? sum.z : 0.0f, sum.w = r + 3 < rank ? sum.w : 0.0f;
+                    lora_put<NT>(hs, lora_pitch<KU>(rank), tok, r, sum);
+                }
             }
             __syncthreads();
         });
@@ -777,7 +803,7 @@ LoraLayout lora_layout(int64_t tokens, int64_t adapters, int64_t max_rank) {
         l.bytes += (n + 15) & ~int64_t{15};
         return at;
     };
-    take(4 * tokens * max_rank * lora_max_splits(static_cast<int>(tokens)));
+    take(4 * tokens * lora_h_pitch(static_cast<int>(max_rank)) * lora_max_splits(static_cast<int>(tokens)));
     if (tokens > kLoraScan) {
         l.tiles = take(sizeof(LoraTile) * lora_most_tiles(tokens, adapters, kLoraTile));
         l.places = take(4 * tokens);
@@ -860,6 +886,8 @@ int32_t lora_launch(LoraArgs &p, bool vec_a, bool vec_b, cudaStream_t stream) {
     p.splits = std::clamp(2 * sms / full, 1, std::min(lora_max_splits(p.tokens), lora_ceil(all_units, 4 * kLoraWarps)));
     p.units = lora_ceil(all_units, p.splits);
     p.splits = lora_ceil(all_units, p.units);
+    const int quads = 8 * NT * lora_ceil(p.max_rank, 16) * 4;  // sums that expand makes of a tile's parts of h
+    while (2 * quads << p.team <= kLoraThreads && 1 << p.team < p.splits) ++p.team;
     const int ranks = p.max_rank <= 16 ? 16 : p.max_rank <= 32 ? 32 : kLoraRankChunk;
     // Two CTAs an SM share the work, whatever the number of tiles turns out to be; fewer where there is less.
     const auto ctas = [&](int64_t items) { return dim3(static_cast<unsigned>(std::min<int64_t>(items * tiles, 2 * sms))); };
