@@ -192,7 +192,8 @@ template <int TILE>
 struct LoraTiles {
     int count;
     int tokens[TILE], adapter, n, rank;  // of the tile last opened
-    int ids[kLoraScan], leads[kLoraScan / 32];
+    alignas(16) int ids[kLoraScan];
+    int leads[kLoraScan / 32];
     int tile_adapter[kLoraScan], tile_n[kLoraScan], tile_rank[kLoraScan], tile_tokens[kLoraScan][TILE];
 };
 
@@ -217,8 +218,12 @@ __device__ __forceinline__ void lora_tiles(LoraTiles<TILE> &s, const LoraArgs &p
     __syncthreads();
     uint64_t same = 0;  // the tokens of this one's adapter
     if (tid < kLoraScan) {
-#pragma unroll 8
-        for (int j = 0; j < kLoraScan; ++j) same |= static_cast<uint64_t>(s.ids[j] == a) << j;
+        for (int j0 = 0; j0 < p.tokens; j0 += 8) {
+            const int4 u = *reinterpret_cast<const int4 *>(s.ids + j0), v = *reinterpret_cast<const int4 *>(s.ids + j0 + 4);
+            const uint32_t m = (u.x == a) | (u.y == a) << 1 | (u.z == a) << 2 | (u.w == a) << 3 | (v.x == a) << 4 |
+                               (v.y == a) << 5 | (v.z == a) << 6 | (v.w == a) << 7;
+            same |= static_cast<uint64_t>(m) << j0;
+        }
         const bool leads = a >= 0 && __popcll(same & ((1ull << tid) - 1)) % TILE == 0;
         const uint32_t m = __ballot_sync(0xffffffffu, leads);
         if (lane == 0) s.leads[warp] = m;
