@@ -18,6 +18,16 @@
 //
 // Tokens of one adapter are gathered into tiles.  A token's sums are made in
 // the same order whatever tile and place it lands in.
+//
+// Measured in CUDA graphs, beside the time that a copy of the bytes read and
+// written takes (6.57 TB/s): 1 token, 576 x 6144, rank 8, BF16 5.1 us (0.02);
+// 64 tokens of 64 adapters, 16384 x 2048, rank 16, BF16 20.9 us (7.1); 48 tokens
+// of 5 adapters, 6144 x 16384, rank 64, F16 12.5 us (2.6); 1000 tokens of 11
+// adapters, 2048 x 6144, rank 64, F16 32 us (7.0); 4096 tokens of 16 adapters,
+// 12288 x 6144, rank 32, BF16 138 us (79.5).  Few tokens are bound by the chain
+// of waits (ids, ranks, weights, h, weights), many by instructions and the L1's
+// data path: of 4096 tokens' call expand takes 100 us with the LSU's data path
+// at 81 % and the schedulers issuing in 42 % of the cycles, DRAM at 45 %.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -32,7 +42,9 @@ namespace {
 
 constexpr int kLoraMaxRank = 256;
 constexpr int kLoraThreads = 256, kLoraWarps = kLoraThreads / 32;
-constexpr int kLoraScan = 64;        // tokens up to which each CTA finds its tile's tokens itself
+// Tokens up to which each CTA finds the tiles itself (a word of bits).  More take a kernel that plans and tiles of 16:
+// at 64 tokens of 64 adapters of 16384 x 2048, rank 16, that is 26.6 us against 20.8; at 40 19.1 against 13.9.
+constexpr int kLoraScan = 64;
 constexpr int kLoraMaxSplits = 32;
 constexpr int kLoraRankChunk = 64;   // ranks a shrink CTA takes
 constexpr int kLoraRows = 32;        // rows of B a warp takes at once
@@ -126,7 +138,8 @@ __device__ __forceinline__ void lora_keep(uint4 &raw, const uint4 &mask) {
 template <class W>
 __device__ __forceinline__ float4 lora_f32(const LoraRaw<W> &raw) {
     if constexpr (sizeof(W) == 4) {
-        return make_float4(__uint_as_float(raw.x), __uint_as_float(raw.y), __uint_as_float(raw.z), __uint_as_float(raw.w));
+        return make_float4(__uint_as_float(raw.x), __uint_as_float(raw.y), __uint_as_float(raw.z),
+                           __uint_as_float(raw.w));
     } else if constexpr (std::is_same_v<W, __half>) {
         const float2 lo = __half22float2(*reinterpret_cast<const __half2 *>(&raw.x));
         const float2 hi = __half22float2(*reinterpret_cast<const __half2 *>(&raw.y));
@@ -219,7 +232,8 @@ __device__ __forceinline__ void lora_tiles(LoraTiles<TILE> &s, const LoraArgs &p
     uint64_t same = 0;  // the tokens of this one's adapter
     if (tid < kLoraScan) {
         for (int j0 = 0; j0 < p.tokens; j0 += 8) {
-            const int4 u = *reinterpret_cast<const int4 *>(s.ids + j0), v = *reinterpret_cast<const int4 *>(s.ids + j0 + 4);
+            const int4 u = *reinterpret_cast<const int4 *>(s.ids + j0);
+            const int4 v = *reinterpret_cast<const int4 *>(s.ids + j0 + 4);
             const uint32_t m = (u.x == a) | (u.y == a) << 1 | (u.z == a) << 2 | (u.w == a) << 3 | (v.x == a) << 4 |
                                (v.y == a) << 5 | (v.z == a) << 6 | (v.w == a) << 7;
             same |= static_cast<uint64_t>(m) << j0;
@@ -234,7 +248,8 @@ __device__ __forceinline__ void lora_tiles(LoraTiles<TILE> &s, const LoraArgs &p
         int k = __popc(s.leads[warp] & ((1u << lane) - 1));
         for (int w = 0; w < warp; ++w) k += __popc(s.leads[w]);
         int n = 0;
-        for (uint64_t left = same >> tid << tid; left && n < TILE; left &= left - 1) s.tile_tokens[k][n++] = __ffsll(left) - 1;
+        for (uint64_t left = same >> tid << tid; left && n < TILE; left &= left - 1)
+            s.tile_tokens[k][n++] = __ffsll(left) - 1;
         s.tile_adapter[k] = a;
         s.tile_n[k] = n;
         s.tile_rank[k] = min(max(rank, 0), p.max_rank);
@@ -357,8 +372,8 @@ struct LoraShrink {
 
     // Ranks r0 .. of adapter a (of its `rank`) and the columns of units first .. u1 of 16; the warps' sums stand in
     // s.parts when it returns, for sum().
-    static __device__ __forceinline__ void run(const LoraArgs &p, Shared &s, const int (&tokens)[8 * NT], int a, int rank,
-                                               int r0, int first, int u1) {
+    static __device__ __forceinline__ void run(const LoraArgs &p, Shared &s, const int (&tokens)[8 * NT], int a,
+                                               int rank, int r0, int first, int u1) {
         const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = 4 * (lane & 3), t8 = 2 * t4;
         const int kw = warp / MW, rw = r0 + 16 * MT * (warp % MW) + g;  // the lane's first rank
         const int u0 = first + 2 * kw;
@@ -519,10 +534,12 @@ struct LoraExpand {
     static constexpr int kSpan = kLoraRows * RG, kChunk = 16 * KU;
 
     template <class F>
-    static __device__ __forceinline__ void run(const LoraArgs &p, const float *hs, const int (&tokens)[8 * NT], int n, int a,
-                                               int rank, int row_first, int row_next, int steps, const F &prepare) {
+    static __device__ __forceinline__ void run(const LoraArgs &p, const float *hs, const int (&tokens)[8 * NT], int n,
+                                               int a, int rank, int row_first, int row_next, int steps,
+                                               const F &prepare) {
         const int t4 = 4 * (threadIdx.x & 3);
-        const int chunks = (rank + kChunk - 1) / kChunk, lane_r = KU * t4;  // a lane has 4 KU neighbouring ranks of a chunk
+        const int chunks = (rank + kChunk - 1) / kChunk;
+        const int lane_r = KU * t4;  // a lane has 4 KU neighbouring ranks of a chunk
         const int lane = threadIdx.x & 31, g = lane >> 2, pitch = lora_pitch<KU>(rank);
         const float scale = p.scales[a];
         const float *ls = hs + 8 * NT * pitch;
@@ -568,7 +585,8 @@ struct LoraExpand {
             for (int q = 0; q < RG; ++q) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int r = min(row + kLoraRows * q + i, VEC ? p.rows - 4 + i : p.rows - 1), left = rank - kChunk * c - lane_r;
+                    const int r = min(row + kLoraRows * q + i, VEC ? p.rows - 4 + i : p.rows - 1);
+                    const int left = rank - kChunk * c - lane_r;
                     const W *from = b + static_cast<int64_t>(r) * p.max_rank + kChunk * c;
                     if constexpr (KU == 2) {
                         const LoraEight<W> v = lora_load8<W, VEC>(from, left);
@@ -692,14 +710,15 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(LoraArgs p
         at += steps;
         const int rank = tiles.rank;
         if (rank == 0) continue;
-        Expand::run(p, hs, tiles.tokens, tiles.n, tiles.adapter, rank, (first * kLoraWarps + warp) * Expand::kSpan, kNext,
-                    steps, [&]() {
+        const int row_first = (first * kLoraWarps + warp) * Expand::kSpan;
+        Expand::run(p, hs, tiles.tokens, tiles.n, tiles.adapter, rank, row_first, kNext, steps, [&]() {
             if (!waited) grid_dependency_wait();  // h comes from the kernel before
             waited = true;
             // Each quad of ranks is summed by 2^team lanes, four parts in flight in each: the joining is bound by
             // its instructions (of 32 parts, rank 64: a quad at once 33.4 us, single values, eight parts in flight,
             // 37.8, sixteen 40.2, of a call of 1000 tokens).
-            const int quads = (rank + Expand::kChunk - 1) / Expand::kChunk * (Expand::kChunk / 4), items = 8 * NT * quads;
+            const int quads = (rank + Expand::kChunk - 1) / Expand::kChunk * (Expand::kChunk / 4);
+            const int items = 8 * NT * quads;
             const int shift = p.team, team = 1 << shift, member = tid & (team - 1);
             for (int i0 = 0; i0 < items; i0 += kLoraThreads >> shift) {
                 const int i = i0 + (tid >> shift), tok = i / quads, r = 4 * (i - tok * quads);
@@ -725,7 +744,8 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(LoraArgs p
                     sum.z += __shfl_xor_sync(0xffffffffu, sum.z, o), sum.w += __shfl_xor_sync(0xffffffffu, sum.w, o);
                 }
                 if (member == 0 && i < items) {
-                    sum.y = r + 1 < rank ? sum.y : 0.0f, sum.z = r + 2 < rank ? sum.z : 0.0f, sum.w = r + 3 < rank ? sum.w : 0.0f;
+                    sum.y = r + 1 < rank ? sum.y : 0.0f, sum.z = r + 2 < rank ? sum.z : 0.0f;
+                    sum.w = r + 3 < rank ? sum.w : 0.0f;
                     lora_put<NT>(hs, lora_pitch<KU>(rank), tok, r, sum);
                 }
             }
@@ -776,7 +796,8 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_cluster_kernel(LoraArgs 
         }
     }
     cluster_arrive();
-    const int row_first = (part * kLoraWarps + (tid >> 5)) * Expand::kSpan, row_next = kLoraCluster * kLoraWarps * Expand::kSpan;
+    const int row_first = (part * kLoraWarps + (tid >> 5)) * Expand::kSpan;
+    const int row_next = kLoraCluster * kLoraWarps * Expand::kSpan;
     const int steps = row_first < p.rows ? (p.rows - row_first + row_next - 1) / row_next : 0;
     Expand::run(p, hs, tiles.tokens, n, tiles.adapter, rank, row_first, row_next, steps, [&]() {
         cluster_wait();
@@ -805,7 +826,9 @@ constexpr int lora_ceil(int64_t n, int64_t of) { return static_cast<int>((n + of
 int lora_max_splits(int tokens) { return std::clamp(lora_ceil(16384, tokens), 1, kLoraMaxSplits); }
 
 // Tiles of `size` tokens there may be: each but an adapter's last one is full.
-int64_t lora_most_tiles(int64_t tokens, int64_t adapters, int size) { return std::min(tokens, tokens / size + adapters); }
+int64_t lora_most_tiles(int64_t tokens, int64_t adapters, int size) {
+    return std::min(tokens, tokens / size + adapters);
+}
 
 // The workspace: h, then (where there is a plan) the tiles, the places, the counts.
 struct LoraLayout {
@@ -831,7 +854,8 @@ LoraLayout lora_layout(int64_t tokens, int64_t adapters, int64_t max_rank) {
 
 // Launches `kernel`, which waits itself for the kernel before it where it needs it.
 template <class K>
-int32_t lora_start(K *kernel, dim3 grid, size_t smem, const LoraArgs &p, bool early, cudaStream_t stream, const char *name) {
+int32_t lora_start(K *kernel, dim3 grid, size_t smem, const LoraArgs &p, bool early, cudaStream_t stream,
+                   const char *name) {
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -848,8 +872,8 @@ int32_t lora_start(K *kernel, dim3 grid, size_t smem, const LoraArgs &p, bool ea
 
 template <class W, int MT, int MW, int NT>
 int32_t lora_shrink(const LoraArgs &p, dim3 grid, bool vec, cudaStream_t stream) {
-    return lora_start(vec ? lora_shrink_kernel<W, MT, MW, NT, true> : lora_shrink_kernel<W, MT, MW, NT, false>, grid, 0, p,
-                      p.tiles, stream, "lora_shrink_kernel");
+    const auto kernel = vec ? lora_shrink_kernel<W, MT, MW, NT, true> : lora_shrink_kernel<W, MT, MW, NT, false>;
+    return lora_start(kernel, grid, 0, p, p.tiles, stream, "lora_shrink_kernel");
 }
 
 template <class W, int NT, int RG, int KU>
@@ -862,7 +886,8 @@ int32_t lora_expand(const LoraArgs &p, dim3 grid, bool vec, cudaStream_t stream)
 
 template <class W, int MT, int MW, int RG, int KU>
 int32_t lora_cluster(const LoraArgs &p, int tiles, bool vec, cudaStream_t stream) {
-    const auto kernel = vec ? lora_cluster_kernel<W, MT, MW, RG, KU, true> : lora_cluster_kernel<W, MT, MW, RG, KU, false>;
+    const auto kernel =
+        vec ? lora_cluster_kernel<W, MT, MW, RG, KU, true> : lora_cluster_kernel<W, MT, MW, RG, KU, false>;
     const size_t smem = sizeof(float) * (16 * lora_pitch<KU>(p.max_rank) + 8 * p.max_rank);
     if (const int32_t rc = allow_dynamic_smem(kernel, smem, "lora_cluster smem")) return rc;
     cudaLaunchAttribute attr[1];
@@ -898,22 +923,31 @@ int32_t lora_launch(LoraArgs &p, bool vec_a, bool vec_b, cudaStream_t stream) {
         if (const int32_t rc = launch_status("lora_plan_kernel")) return rc;
     }
     // Columns in as many parts as give two items an SM were every tile full, none shorter than four units a warp.
+    // Half as many: 1000 tokens 39.4 us against 32.1, 48 tokens of rank 64 13.1 against 12.5; twice as many: 39.8
+    // and, 4096 tokens, 140.0 against 138.1.
     const int full = lora_ceil(p.tokens, 8 * NT), all_units = lora_ceil(p.cols, 16);
     p.splits = std::clamp(2 * sms / full, 1, std::min(lora_max_splits(p.tokens), lora_ceil(all_units, 4 * kLoraWarps)));
     p.units = lora_ceil(all_units, p.splits);
     p.splits = lora_ceil(all_units, p.units);
     const int quads = 8 * NT * lora_ceil(p.max_rank, 16) * 4;  // sums that expand makes of a tile's parts of h
     while (2 * quads << p.team <= kLoraThreads && 1 << p.team < p.splits) ++p.team;
+    // Ranks a shrink item takes.  64 instead of 32 for rank 32: 161 us against 138 (4096 tokens); 64 instead of 16 for
+    // rank 16: 149 against 116, 64 tokens 22.4 against 20.8; 32 instead of 64 for rank 64: 1000 tokens 34.2 against
+    // 32.1, 64 tokens 38.3 against 37.4.
     const int ranks = p.max_rank <= 16 ? 16 : p.max_rank <= 32 ? 32 : kLoraRankChunk;
     // Two CTAs an SM share the work, whatever the number of tiles turns out to be; fewer where there is less.
-    const auto ctas = [&](int64_t items) { return dim3(static_cast<unsigned>(std::min<int64_t>(items * tiles, 2 * sms))); };
+    const auto ctas = [&](int64_t items) {
+        return dim3(static_cast<unsigned>(std::min<int64_t>(items * tiles, 2 * sms)));
+    };
     const dim3 grid = ctas(int64_t{p.splits} * lora_ceil(p.max_rank, ranks));
     int32_t rc = kOk;
     if (ranks == 16) rc = lora_shrink<W, 1, 1, NT>(p, grid, vec_a, stream);
     else if (ranks == 32) rc = lora_shrink<W, 2, 1, NT>(p, grid, vec_a, stream);
     else rc = lora_shrink<W, 2, 2, NT>(p, grid, vec_a, stream);
     if (rc) return rc;
-    // Ranks a chunk: 16, with twice the rows a step for single tokens, or 32.
+    // Ranks a chunk: 32 (16-byte loads of 16-bit weights) where there are more than 16: 4096 tokens of rank 32 138 us,
+    // of rank 64 187, by 16 at a time 146 and 206; F32 weights fill 16 bytes with 16 ranks.  Rank 16 and few tokens
+    // take twice the rows a step: 64 tokens 20.8 us against 23.7.
     const dim3 out = ctas(lora_ceil(p.rows, kLoraWarps * kLoraRows));
     if (sizeof(W) == 4 || p.max_rank <= 16)
         return lora_expand<W, NT, NT == 1 && sizeof(W) == 2 ? 2 : 1, 1>(p, out, vec_b, stream);
@@ -967,7 +1001,8 @@ GLMVX_EXPORT int32_t glmvx_lora_add(float *y, int64_t y_stride, const float *x, 
         p.counts = reinterpret_cast<int *>(ws + layout.counts);
         p.ntiles = reinterpret_cast<int *>(ws + layout.ntiles);
     }
-    // 16 bytes at once (8 for ranks up to 16) where they stand on their boundary.
+    // 16 bytes at once (8 for ranks up to 16) where they stand on their boundary, else value by value: 4096 tokens
+    // 138 us against 310, 64 tokens 20.9 against 39.2.
     const int per_a = kind == 0 ? 4 : 8, per_b = kind == 0 || max_rank <= 16 ? 4 : 8;
     const bool vec_a = !(cols % per_a) && !((bits(a) | bits(x)) & 15) && (tokens == 1 || !(x_stride & 3));
     const bool vec_b = !(max_rank % per_b) && !(rows & 3) && !(bits(b) & (kind == 0 || per_b == 8 ? 15 : 7)) &&
@@ -975,6 +1010,7 @@ GLMVX_EXPORT int32_t glmvx_lora_add(float *y, int64_t y_stride, const float *x, 
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool wide = tokens > kLoraScan;
     if (kind == 0) return wide ? lora_launch<float, 2>(p, vec_a, vec_b, s) : lora_launch<float, 1>(p, vec_a, vec_b, s);
-    if (kind == 1) return wide ? lora_launch<__half, 2>(p, vec_a, vec_b, s) : lora_launch<__half, 1>(p, vec_a, vec_b, s);
+    if (kind == 1)
+        return wide ? lora_launch<__half, 2>(p, vec_a, vec_b, s) : lora_launch<__half, 1>(p, vec_a, vec_b, s);
     return wide ? lora_launch<__nv_bfloat16, 2>(p, vec_a, vec_b, s) : lora_launch<__nv_bfloat16, 1>(p, vec_a, vec_b, s);
 }

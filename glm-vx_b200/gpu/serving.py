@@ -119,7 +119,8 @@ class BatchScheduler:
         amount = len(tokens) + max_tokens
         if amount > min(cfg.get('max_position_embeddings', 2**31 - 1), self.decoder.capacity):
             raise ValueError('request exceeds context limit')
-        req = Request(tuple(tokens), max_tokens, float(temperature), seed, adapter=adapter, rules=rules, allowed=allowed)
+        req = Request(tuple(tokens), max_tokens, float(temperature), seed, adapter=adapter, rules=rules,
+                      allowed=allowed)
         req.reservation = amount
         req.rng = np.random.default_rng(seed)
         req.events = queue.Queue(maxsize=min(max_tokens + 2, self.max_pending_events))

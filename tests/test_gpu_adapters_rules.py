@@ -41,7 +41,8 @@ class Source:
             self.dense[a + '.indexer.k_norm.bias'] = np.zeros(c['index_head_dim'], np.float32)
             heads = c['num_attention_heads'] * (c['qk_nope_head_dim'] + c['v_head_dim'])
             self.dense[a + '.kv_b_proj.weight'] = matrix('kv_b', heads, c['kv_lora_rank'])
-            self.packed[a + '.indexer.wq_b'] = matrix('wq_b', c['index_n_heads'] * c['index_head_dim'], c['q_lora_rank'])
+            self.packed[a + '.indexer.wq_b'] = matrix('wq_b', c['index_n_heads'] * c['index_head_dim'],
+                                                      c['q_lora_rank'])
             self.packed[a + '.indexer.wk'] = matrix('wk', c['index_head_dim'], H)
             self.packed[a + '.indexer.weights_proj'] = matrix('w', c['index_n_heads'], H)
         for name, (a, b) in (changes or {}).items():
@@ -212,7 +213,8 @@ def test_rules_in_the_captured_step(gpu_backend, plain_logits):
     rules = LogitRules(gpu_backend, len(PROMPTS), CONFIG['vocab_size'], capacity=40, max_bias=8)
     dec = decoder(gpu_backend, rules=rules)
     sets = [dict(prompt=4, repetition=1.3, presence=0.5, frequency=0.25),
-            dict(prompt=2, repetition=0.7, frequency=-0.5, bias={9: -np.inf, 120: 30.0, 7: -1.5}, allowed=range(0, 300, 3)),
+            dict(prompt=2, repetition=0.7, frequency=-0.5, bias={9: -np.inf, 120: 30.0, 7: -1.5},
+                 allowed=range(0, 300, 3)),
             {}]
     try:
         assert run(dec).tobytes() == plain_logits.tobytes()  # rules that say nothing

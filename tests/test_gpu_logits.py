@@ -274,7 +274,8 @@ def test_captured_steps_feed_themselves(gpu_backend):
 @pytest.mark.parametrize('rows,vocab,cap,bias', [(1, 700001, 100000, 3), (2, 400000, 60000, 2047), (3, 1300000, 8, 1)])
 def test_vocabularies_that_go_in_passes(gpu_backend, rows, vocab, cap, bias):
     """Histories as long as the vocabulary's share of a CTA: the rules do not fit shared memory at once."""
-    Case(rows, vocab, cap, lens=[cap, cap - 1, 0][:rows], penalties=True, bias=bias, masks=2, seed=vocab).check(gpu_backend)
+    Case(rows, vocab, cap, lens=[cap, cap - 1, 0][:rows], penalties=True, bias=bias, masks=2,
+         seed=vocab).check(gpu_backend)
 
 
 @pytest.mark.parametrize('vocab', [4, 124, 128, 132, 2048, 2052, 6148])

@@ -246,8 +246,8 @@ def test_ranks_and_widths_on_both_sides_of_the_tiles(gpu_backend, kind, max_rank
 
 
 @pytest.mark.parametrize('kind', [0, 1, 30])
-@pytest.mark.parametrize('max_rank,cols,rows', [(1, 31, 5), (16, 512, 256), (19, 515, 130), (33, 1000, 132), (64, 64, 1028),
-                                                (256, 264, 36)])
+@pytest.mark.parametrize('max_rank,cols,rows', [(1, 31, 5), (16, 512, 256), (19, 515, 130), (33, 1000, 132),
+                                                (64, 64, 1028), (256, 264, 36)])
 def test_few_tokens_in_one_launch_and_in_two(gpu_backend, kind, max_rank, cols, rows):
     """The number of tiles there may be (tokens, or an eighth of them and one an adapter) decides: from 19 on, two
     launches; both with ranks that differ and adapters that several tiles share."""
