@@ -123,7 +123,8 @@ class AdapterBank:
         """Fills `slot` with an adapter: weights {name: (A [r, cols], B [rows,
         r])} with 0 <= r <= max_rank, the same scale (alpha / r of the usual
         convention) for all of them; projections without an entry are left
-        as the model has them."""
+        as the model has them.  Steps that run meanwhile see the slot empty,
+        then with the projections that are already there."""
         slot = self._slot(slot)
         scale = float(scale)
         if not np.isfinite(scale):

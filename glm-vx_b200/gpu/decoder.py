@@ -149,6 +149,9 @@ class ResidentDecoder:
         self.indexer_types, self.mlp_types = self.indexer_types[:self.n_layers], self.mlp_types[:self.n_layers]
         if self.indexer_types[0] != 'full':
             raise ValueError('the first layer must have a full indexer')
+        for part in (adapters, rules):
+            if part is not None and part.backend is not backend:  # another device's memory, or another stream's order
+                raise ValueError('the adapters and the rules must belong to the decoder\'s backend')
         if rules is not None and (rules.batch, rules.vocab) != (self.B, self.vocab):
             raise ValueError(f'rules are for {rules.batch} sequences over {rules.vocab} tokens, '
                              f'not {self.B} over {self.vocab}')

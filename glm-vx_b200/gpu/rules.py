@@ -37,8 +37,9 @@ def pack_mask(allowed, vocab):
 
 class LogitRules:
     """Rules of `batch` sequences over `vocab` tokens, with histories of up to
-    `capacity` tokens and up to `max_bias` biased tokens each.  A sequence
-    without rules gets the plain argmax (-1 when nothing is above -inf)."""
+    `capacity` tokens (what is fed after that is not remembered) and up to
+    `max_bias` biased tokens each.  A sequence without rules gets the plain
+    argmax (-1 when nothing is above -inf)."""
 
     def __init__(self, backend, batch, vocab, capacity, max_bias=512):
         self.batch, self.vocab = int(batch), int(vocab)

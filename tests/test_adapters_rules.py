@@ -1,6 +1,8 @@
 """Adapter banks, logit rules and the scheduler's use of them, without a GPU:
 argument checks, storage rounding, masks, and the serving loop over a decoder
 that applies the rules in NumPy."""
+from types import SimpleNamespace
+
 import numpy as np
 import pytest
 
@@ -62,6 +64,16 @@ def bank_without_device():
 def test_load_refusals(slot, weights, scale, message):
     with pytest.raises(ValueError, match=message):
         bank_without_device().load(slot, weights, scale)
+
+
+@pytest.mark.parametrize('part', ['adapters', 'rules'])
+def test_a_decoder_refuses_what_belongs_to_another_backend(part):
+    from gpu.decoder import ResidentDecoder
+    config = dict(CONFIG, index_n_heads=2, index_head_dim=16, index_topk=8, indexer_types=['full', 'full'])
+    theirs = dict(adapters=SimpleNamespace(backend=NoDevice(), shapes={}, max_tokens=2, slots=2),
+                  rules=SimpleNamespace(backend=NoDevice(), batch=2, vocab=50))
+    with pytest.raises(ValueError, match='backend'):
+        ResidentDecoder(NoDevice(), config, None, batch=2, capacity=8, **{part: theirs[part]})
 
 
 def test_storage_rounding():
