@@ -961,7 +961,8 @@ int32_t lora_launch(LoraArgs &p, bool vec_a, bool vec_b, cudaStream_t stream) {
 using namespace glmvx;
 
 GLMVX_EXPORT int64_t glmvx_lora_workspace_bytes(int32_t tokens, int32_t adapters, int32_t max_rank) {
-    if (tokens < 0 || tokens > 1 << 20 || adapters < 1 || max_rank < 1 || max_rank > kLoraMaxRank) return kInvalid;
+    if (tokens < 0 || tokens > 1 << 20 || adapters < 1 || adapters > 1 << 24 || max_rank < 1 || max_rank > kLoraMaxRank)
+        return kInvalid;
     return lora_layout(tokens, adapters, max_rank).bytes;
 }
 
@@ -970,7 +971,8 @@ GLMVX_EXPORT int32_t glmvx_lora_add(float *y, int64_t y_stride, const float *x, 
                                     const int32_t *ranks, const float *scales, int32_t tokens, int32_t rows,
                                     int32_t cols, int32_t adapters, int32_t max_rank, void *workspace,
                                     uint64_t workspace_bytes, void *stream) {
-    if (tokens < 0 || tokens > 1 << 20 || rows < 1 || cols < 1 || adapters < 1 || rows > 1 << 22 || cols > 1 << 22)
+    if (tokens < 0 || tokens > 1 << 20 || rows < 1 || cols < 1 || adapters < 1 || rows > 1 << 22 || cols > 1 << 22 ||
+        adapters > 1 << 24)
         return set_error("lora_add: invalid dimensions"), kInvalid;
     if (max_rank < 1 || max_rank > kLoraMaxRank)
         return set_error("lora_add: max_rank must be 1..%d", kLoraMaxRank), kInvalid;

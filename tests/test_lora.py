@@ -16,6 +16,7 @@ def call(**change):
 @pytest.mark.parametrize('change,code,message', [
     (dict(tokens=-1), -1, 'dimensions'), (dict(tokens=(1 << 20) + 1), -1, 'dimensions'),
     (dict(rows=0), -1, 'dimensions'), (dict(cols=0), -1, 'dimensions'), (dict(adapters=0), -1, 'dimensions'),
+    (dict(adapters=(1 << 24) + 1), -1, 'dimensions'),
     (dict(rows=(1 << 22) + 1), -1, 'dimensions'), (dict(cols=(1 << 22) + 1), -1, 'dimensions'),
     (dict(max_rank=0), -1, 'max_rank'), (dict(max_rank=257), -1, 'max_rank'), (dict(kind=8), -4, 'kind'),
     (dict(kind=-1), -4, 'kind'), (dict(y_stride=63), -1, 'strides'), (dict(x_stride=31), -1, 'strides'),
@@ -37,5 +38,5 @@ def test_workspace_size():
     size = rt.library().glmvx_lora_workspace_bytes
     assert size(1, 1, 1) > 0 and size(0, 1, 1) > 0
     assert size(64, 4, 16) >= 64 * 16 * 4
-    for bad in ((-1, 1, 1), ((1 << 20) + 1, 1, 1), (1, 0, 1), (1, 1, 0), (1, 1, 257)):
+    for bad in ((-1, 1, 1), ((1 << 20) + 1, 1, 1), (1, 0, 1), (1, (1 << 24) + 1, 1), (1, 1, 0), (1, 1, 257)):
         assert size(*bad) < 0
