@@ -115,9 +115,10 @@ class AdapterBank:
         return slot
 
     def _put(self, buf, array, offset):
-        self.backend.stream.synchronize()  # steps in flight still read what is there
-        buf.upload(array, self.backend.stream.handle, offset)
-        self.backend.stream.synchronize()
+        with self.backend.device.lock:  # no other thread captures a step on the stream meanwhile
+            self.backend.stream.synchronize()  # steps in flight still read what is there
+            buf.upload(array, self.backend.stream.handle, offset)
+            self.backend.stream.synchronize()
 
     def load(self, slot, weights, scale=1.0):
         """Fills `slot` with an adapter: weights {name: (A [r, cols], B [rows,

@@ -476,11 +476,12 @@ class ResidentDecoder:
     def step_graph(self):
         if self._graph is None:
             g = rt.Graph(self.backend.stream)
-            g.begin()
-            try:
-                self._step_launches()
-            finally:
-                g.end()
+            with self.backend.device.lock:  # an adapter loaded by another thread meanwhile would end up in the graph
+                g.begin()
+                try:
+                    self._step_launches()
+                finally:
+                    g.end()
             self._graph = g
         return self._graph
 
@@ -549,9 +550,10 @@ class ResidentDecoder:
                 raise ValueError('the decoder has no adapter bank')
             if type(slot) is not int or not 0 <= slot < self.adapters.slots or not self.adapters.loaded[slot]:
                 raise ValueError('no adapter is loaded there')
-        self.backend.stream.synchronize()  # the step in flight has read the ids
-        self.adapter_ids.upload(np.array([-1 if slot is None else slot], np.int32), self.s, 4 * b)
-        self.backend.stream.synchronize()
+        with self.backend.device.lock:
+            self.backend.stream.synchronize()  # the step in flight has read the ids
+            self.adapter_ids.upload(np.array([-1 if slot is None else slot], np.int32), self.s, 4 * b)
+            self.backend.stream.synchronize()
 
     def reset_slot(self, b):
         """Empty sequence b's caches in every layer (its length to 0); with

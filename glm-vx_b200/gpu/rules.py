@@ -63,9 +63,10 @@ class LogitRules:
     def _put(self, name, array, item, width=1):
         """`array` into element `item` of buffer `name` (elements of `width` words)."""
         s = self.backend.stream
-        s.synchronize()  # a step in flight still reads what is there
-        self._bufs[name].upload(np.ascontiguousarray(array), s.handle, 4 * item * width)
-        s.synchronize()
+        with self.backend.device.lock:  # no other thread captures a step on the stream meanwhile
+            s.synchronize()  # a step in flight still reads what is there
+            self._bufs[name].upload(np.ascontiguousarray(array), s.handle, 4 * item * width)
+            s.synchronize()
 
     def _sequence(self, b):
         if not 0 <= b < self.batch:
@@ -128,13 +129,14 @@ class LogitRules:
         """The tokens sequence b has been fed."""
         self._sequence(b)
         lens = np.empty(self.batch, np.int32)
-        self.backend.stream.synchronize()
-        self._bufs['lens'].download(lens, self.backend.stream.handle)
-        self.backend.stream.synchronize()
-        row = np.empty(int(lens[b]), np.int32)
-        if row.size:
-            self._bufs['history'].download(row, self.backend.stream.handle, 4 * b * self.capacity)
+        with self.backend.device.lock:
             self.backend.stream.synchronize()
+            self._bufs['lens'].download(lens, self.backend.stream.handle)
+            self.backend.stream.synchronize()
+            row = np.empty(int(lens[b]), np.int32)
+            if row.size:
+                self._bufs['history'].download(row, self.backend.stream.handle, 4 * b * self.capacity)
+                self.backend.stream.synchronize()
         return row
 
     def select(self, tokens, logits, stream=None):

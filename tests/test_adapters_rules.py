@@ -76,6 +76,59 @@ def test_a_decoder_refuses_what_belongs_to_another_backend(part):
         ResidentDecoder(NoDevice(), config, None, batch=2, capacity=8, **{part: theirs[part]})
 
 
+class CountingLock:
+    depth = 0
+
+    def __enter__(self):
+        self.depth += 1
+
+    def __exit__(self, *exc):
+        self.depth -= 1
+
+
+class QuietBackend:
+    """A backend that only notes whether the device's lock was held."""
+
+    def __init__(self):
+        self.device, self.held = SimpleNamespace(lock=CountingLock()), []
+        self.stream = SimpleNamespace(handle=0, synchronize=self._note)
+
+    def _note(self, *args):
+        self.held.append(self.device.lock.depth > 0)
+
+    def _begin(self):
+        pass
+
+    def buffer(self):
+        return SimpleNamespace(ptr=0, upload=self._note)
+
+
+def test_what_is_put_into_place_waits_for_a_capture(monkeypatch):
+    """Loading an adapter or a rule works on the stream that another thread may be capturing a step on: both hold the
+    device's lock."""
+    from gpu import decoder
+    from gpu import runtime as rt
+    backend = QuietBackend()
+    bank = bank_without_device()
+    bank.backend, bank._stacks = backend, {'a': tuple(backend.buffer() for _ in range(4))}
+    bank.load(0, {'a': (np.zeros((1, 4)), np.zeros((6, 1)))})
+    assert len(backend.held) >= 12 and all(backend.held)
+    backend.held.clear()
+    rules = LogitRules.__new__(LogitRules)
+    rules.backend, rules.batch, rules.vocab, rules.max_bias, rules.words = backend, 2, 50, 4, 2
+    rules._masked = [None, None]
+    rules._bufs = {n: backend.buffer() for n in ('lens', 'prompts', 'penalties', 'bias_ids', 'bias_values', 'bias_lens',
+                                                 'masks', 'mask_rows')}
+    rules.set(1, bias={3: 1.0}, allowed=[1, 2])
+    assert len(backend.held) >= 12 and all(backend.held)
+    backend.held.clear()
+    dec = decoder.ResidentDecoder.__new__(decoder.ResidentDecoder)
+    dec.backend, dec._graph, dec._step_launches, dec._bufs = backend, None, backend._note, []
+    monkeypatch.setattr(rt, 'Graph', lambda stream: SimpleNamespace(begin=backend._note, end=backend._note))
+    dec.step_graph()
+    assert backend.held == [True] * 3 and backend.device.lock.depth == 0
+
+
 def test_storage_rounding():
     x = np.array([1.0, 1 + 2.0**-8, 1 + 3 * 2.0**-8, -1 - 2.0**-8 - 2.0**-20, 2.0**-130, 0.0], np.float32)
     got = (to_kind(x, 30).astype(np.uint32) << 16).view(np.float32)

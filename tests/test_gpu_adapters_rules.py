@@ -172,6 +172,38 @@ def test_stored_kinds(gpu_backend, plain_logits, kind, step):
         bank.close()
 
 
+def test_an_adapter_loaded_while_the_step_is_captured(gpu_backend, plain_logits):
+    """Another thread's load waits for the capture's end: the graph holds the step alone, the adapter is there after."""
+    import threading
+    import time
+    from gpu.adapters import AdapterBank, projection_shapes
+    bank = AdapterBank(gpu_backend, projection_shapes(CONFIG), slots=1, max_rank=4, kind=0, max_tokens=len(PROMPTS))
+    weights = adapter(3, all_names(), 4)
+    loader = threading.Thread(target=bank.load, args=(0, weights, SCALE))
+    dec = decoder(gpu_backend, adapters=bank)
+    launches = dec._step_launches
+
+    def captured():
+        loader.start()
+        time.sleep(0.3)
+        assert loader.is_alive() and not bank.loaded[0]
+        launches()
+
+    dec._step_launches = captured
+    try:
+        assert run(dec).tobytes() == plain_logits.tobytes()
+        loader.join(10)
+        assert bank.loaded[0]
+        dec.set_adapter(1, 0)
+        got = run(dec)
+        assert run(dec).tobytes() == got.tobytes()
+        assert np.delete(got, 1, axis=1).tobytes() == np.delete(plain_logits, 1, axis=1).tobytes()
+        assert (np.linalg.norm(got[:, 1] - plain_logits[:, 1], axis=-1) > 0.01).all()
+    finally:
+        dec.close()
+        bank.close()
+
+
 def test_decoder_refuses_what_does_not_fit(gpu_backend):
     from gpu.adapters import AdapterBank
     from gpu.rules import LogitRules
