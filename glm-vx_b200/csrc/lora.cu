@@ -67,56 +67,95 @@ struct LoraArgs {
     int *counts, *places, *ntiles;
     int64_t y_stride, x_stride;
     int tokens, rows, cols, adapters, max_rank, splits, units, team;
+    int how_a, how_b, how_x, how_y;  // LoraHow: how rows that are not all on 16-byte boundaries are read
     int *err;
 };
 
 __host__ __device__ constexpr int lora_h_pitch(int max_rank) { return (max_rank + 3) & ~3; }
 __device__ __forceinline__ int lora_rank(const LoraArgs &p, int a) { return min(max(p.ranks[a], 0), p.max_rank); }
 
-// Four neighbouring values as they stand in memory; those from `n` on are 0
-// (n <= 0: nothing is read).  With VEC n is never 1 to 3.
+// N neighbouring values (4 or 8) as they stand in memory.  With VEC they are on their boundary and are read where
+// n > 0.  Without it only n values may be read there, and those from n on are 0: 16 bytes at once where they are on
+// that boundary, else (16-bit) four at once on theirs, else by the words of two that hold them, which has to leave
+// one value behind them; else value by value.  1000 tokens, 2050 x 6146, rank 37: 66 us, value by value 88; 4096
+// tokens, 12288 x 6144, rank 31: 194 us, value by value 244.
 template <class W>
 using LoraRaw = std::conditional_t<sizeof(W) == 4, uint4, uint2>;
 
-template <class W, bool VEC>
-__device__ __forceinline__ LoraRaw<W> lora_load4(const W *w, int n) {
-    LoraRaw<W> raw{};
-    if constexpr (VEC) {
-        if (n > 0) raw = __ldg(reinterpret_cast<const LoraRaw<W> *>(w));
-    } else if constexpr (sizeof(W) == 4) {
-        const uint32_t *v = reinterpret_cast<const uint32_t *>(w);
-        if (n > 0) raw.x = __ldg(v);
-        if (n > 1) raw.y = __ldg(v + 1);
-        if (n > 2) raw.z = __ldg(v + 2);
-        if (n > 3) raw.w = __ldg(v + 3);
-    } else {
-        const uint16_t *v = reinterpret_cast<const uint16_t *>(w);
-        if (n > 0) raw.x = __ldg(v);
-        if (n > 1) raw.x |= static_cast<uint32_t>(__ldg(v + 1)) << 16;
-        if (n > 2) raw.y = __ldg(v + 2);
-        if (n > 3) raw.y |= static_cast<uint32_t>(__ldg(v + 3)) << 16;
-    }
-    return raw;
-}
+enum LoraHow : int { kLoraSingle, kLoraWords, kLoraQuads, kLoraWhole };
 
-// Eight neighbouring values (with VEC on their 16-byte boundary), read where n > 0; without VEC those from n on are 0.
 template <class W>
 struct LoraEight {
     LoraRaw<W> q[2];
 };
 
+template <class T>
+__device__ __forceinline__ T lora_as(const void *from) {
+    return __ldg(static_cast<const T *>(from));
+}
+
+// Words 0 .. N - 1 of the 2 N values of 16 bits at w.
+template <int N>
+__device__ __forceinline__ void lora_words(uint32_t (&to)[N], const void *w) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(w);
+    const uint32_t *from = reinterpret_cast<const uint32_t *>(at & ~uintptr_t{3});
+    const uint32_t shift = (at & 2) * 8;
+    uint32_t u[N + 1];
+#pragma unroll
+    for (int k = 0; k < N; ++k) u[k] = __ldg(from + k);
+    u[N] = shift ? __ldg(from + N) : 0;
+#pragma unroll
+    for (int k = 0; k < N; ++k) to[k] = __funnelshift_r(u[k], u[k + 1], shift);
+}
+
 template <class W, bool VEC>
-__device__ __forceinline__ LoraEight<W> lora_load8(const W *w, int n) {
-    LoraEight<W> v{};
-    if constexpr (VEC && sizeof(W) == 2) {
-        if (n > 0) {
-            const uint4 u = __ldg(reinterpret_cast<const uint4 *>(w));
-            v.q[0] = make_uint2(u.x, u.y), v.q[1] = make_uint2(u.z, u.w);
+__device__ __forceinline__ LoraRaw<W> lora_load4(const W *w, int n, int how) {
+    LoraRaw<W> raw{};
+    if constexpr (VEC) {
+        if (n > 0) raw = lora_as<LoraRaw<W>>(w);
+    } else if constexpr (sizeof(W) == 4) {
+        if (n >= 4 && how == kLoraWhole) {
+            raw = lora_as<uint4>(w);
+        } else {
+            if (n > 0) raw.x = lora_as<uint32_t>(w);
+            if (n > 1) raw.y = lora_as<uint32_t>(w + 1);
+            if (n > 2) raw.z = lora_as<uint32_t>(w + 2);
+            if (n > 3) raw.w = lora_as<uint32_t>(w + 3);
         }
+    } else if (n >= 4 && how >= kLoraQuads) {
+        raw = lora_as<uint2>(w);
+    } else if (n >= 5 && how == kLoraWords) {
+        uint32_t u[2];
+        lora_words(u, w);
+        raw = make_uint2(u[0], u[1]);
     } else {
-        v.q[0] = lora_load4<W, VEC>(w, n);
-        v.q[1] = lora_load4<W, VEC>(w + 4, n - 4);
+        if (n > 0) raw.x = lora_as<uint16_t>(w);
+        if (n > 1) raw.x |= static_cast<uint32_t>(lora_as<uint16_t>(w + 1)) << 16;
+        if (n > 2) raw.y = lora_as<uint16_t>(w + 2);
+        if (n > 3) raw.y |= static_cast<uint32_t>(lora_as<uint16_t>(w + 3)) << 16;
     }
+    return raw;
+}
+
+template <class W, bool VEC>
+__device__ __forceinline__ LoraEight<W> lora_load8(const W *w, int n, int how) {
+    LoraEight<W> v{};
+    if constexpr (sizeof(W) == 2) {
+        if (VEC ? n > 0 : n >= 8 && how == kLoraWhole) {
+            const uint4 u = lora_as<uint4>(w);
+            v.q[0] = make_uint2(u.x, u.y), v.q[1] = make_uint2(u.z, u.w);
+            return v;
+        }
+        if constexpr (VEC) return v;
+        if (n >= 9 && how == kLoraWords) {
+            uint32_t u[4];
+            lora_words(u, w);
+            v.q[0] = make_uint2(u[0], u[1]), v.q[1] = make_uint2(u[2], u[3]);
+            return v;
+        }
+    }
+    v.q[0] = lora_load4<W, VEC>(w, n, how);
+    v.q[1] = lora_load4<W, VEC>(w + 4, n - 4, how);
     return v;
 }
 
@@ -320,7 +359,7 @@ __global__ void __launch_bounds__(kLoraPlanThreads) lora_plan_kernel(LoraArgs p)
         p.places[t] = a >= 0 && a < p.adapters ? atomicAdd(counts + a, 1) : 0;
     }
     __syncthreads();
-    int base = 0;  // the tiles of the adapters before this round's
+    int base = 0;  // the tiles of the adapters before these
     for (int a0 = 0; a0 < p.adapters; a0 += kLoraPlanThreads) {
         const int a = a0 + tid, n = a < p.adapters ? counts[a] : 0, nt = (n + kLoraTile - 1) / kLoraTile;
         if (a0) rank = a < p.adapters ? lora_rank(p, a) : 0;
@@ -389,9 +428,9 @@ struct LoraShrink {
         float acc[MT][NT][4] = {};
         const auto load = [&](Batch &t, int left) {  // left: columns from the lane's first to the end of the split
 #pragma unroll
-            for (int j = 0; j < NT; ++j) t.x[j] = lora_load8<float, VEC>(x[j], left), x[j] += kBatch;
+            for (int j = 0; j < NT; ++j) t.x[j] = lora_load8<float, VEC>(x[j], left, p.how_x), x[j] += kBatch;
 #pragma unroll
-            for (int i = 0; i < 2 * MT; ++i) t.w[i] = lora_load8<W, VEC>(w[i], left), w[i] += kBatch;
+            for (int i = 0; i < 2 * MT; ++i) t.w[i] = lora_load8<W, VEC>(w[i], left, p.how_a), w[i] += kBatch;
         };
         const auto multiply = [&](const Batch &t) {
 #pragma unroll
@@ -544,6 +583,7 @@ struct LoraExpand {
         const float scale = p.scales[a];
         const float *ls = hs + 8 * NT * pitch;
         const W *b = static_cast<const W *>(p.b) + static_cast<int64_t>(a) * p.rows * p.max_rank + lane_r;
+        const W *b_end = static_cast<const W *>(p.b) + static_cast<int64_t>(p.adapters) * p.rows * p.max_rank;
         float *y[NT][2];  // the lane's tokens' rows
         bool mine[NT][2];
 #pragma unroll
@@ -572,6 +612,8 @@ struct LoraExpand {
                         if (VEC) {
                             *reinterpret_cast<float4 *>(to.v[q][j][e]) =
                                 *reinterpret_cast<const float4 *>(y[j][e] + min(r, p.rows - 4));
+                        } else if (p.how_y == kLoraWhole && r + 4 <= p.rows) {
+                            *reinterpret_cast<float4 *>(to.v[q][j][e]) = *reinterpret_cast<const float4 *>(y[j][e] + r);
                         } else {
 #pragma unroll
                             for (int i = 0; i < 4; ++i) to.v[q][j][e][i] = y[j][e][min(r + i, p.rows - 1)];
@@ -586,13 +628,15 @@ struct LoraExpand {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int r = min(row + kLoraRows * q + i, VEC ? p.rows - 4 + i : p.rows - 1);
-                    const int left = rank - kChunk * c - lane_r;
                     const W *from = b + static_cast<int64_t>(r) * p.max_rank + kChunk * c;
+                    // Behind the rank others' values may be read, up to the stack's end: the last chunk's mask drops them.
+                    int n = rank - kChunk * c - lane_r;
+                    if (!VEC && n > 0) n = static_cast<int>(min(b_end - from, static_cast<ptrdiff_t>(16)));
                     if constexpr (KU == 2) {
-                        const LoraEight<W> v = lora_load8<W, VEC>(from, left);
+                        const LoraEight<W> v = lora_load8<W, VEC>(from, n, p.how_b);
                         to.w[0][q][i] = v.q[0], to.w[1][q][i] = v.q[1];
                     } else {
-                        to.w[0][q][i] = lora_load4<W, VEC>(from, left);
+                        to.w[0][q][i] = lora_load4<W, VEC>(from, n, p.how_b);
                     }
                 }
             }
@@ -669,7 +713,7 @@ struct LoraExpand {
                         const float *o = old.v[q][j][e];
                         const float v[4] = {fmaf(scale, acc[q][0][j][e], o[0]), fmaf(scale, acc[q][0][j][2 + e], o[1]),
                                             fmaf(scale, acc[q][1][j][e], o[2]), fmaf(scale, acc[q][1][j][2 + e], o[3])};
-                        if (VEC) {
+                        if (VEC || (p.how_y == kLoraWhole && r + 4 <= p.rows)) {
                             if (mine[j][e] && r < p.rows)
                                 *reinterpret_cast<float4 *>(y[j][e] + r) = make_float4(v[0], v[1], v[2], v[3]);
                         } else {
@@ -1003,12 +1047,18 @@ GLMVX_EXPORT int32_t glmvx_lora_add(float *y, int64_t y_stride, const float *x, 
         p.counts = reinterpret_cast<int *>(ws + layout.counts);
         p.ntiles = reinterpret_cast<int *>(ws + layout.ntiles);
     }
-    // 16 bytes at once (8 for ranks up to 16) where they stand on their boundary, else value by value: 4096 tokens
-    // 138 us against 310, 64 tokens 20.9 against 39.2.
-    const int per_a = kind == 0 ? 4 : 8, per_b = kind == 0 || max_rank <= 16 ? 4 : 8;
-    const bool vec_a = !(cols % per_a) && !((bits(a) | bits(x)) & 15) && (tokens == 1 || !(x_stride & 3));
-    const bool vec_b = !(max_rank % per_b) && !(rows & 3) && !(bits(b) & (kind == 0 || per_b == 8 ? 15 : 7)) &&
-                       !(bits(y) & 15) && (tokens == 1 || !(y_stride & 3));
+    // What stands on 16-byte boundaries (8 for ranks up to 16) has kernels of its own, the rest asks how it is read:
+    // 4096 tokens of rank 32 138 us, of rank 28 (quads) 158 and 31 (words) 193, all value by value 310.
+    const int size = kind == 0 ? 4 : 2, per_b = kind == 0 || max_rank <= 16 ? 4 : 8;
+    const auto how = [&](const void *base, int64_t pitch, int each, int group) {
+        if (!(bits(base) & (group * each - 1)) && !(pitch % group)) return kLoraWhole;
+        if (each == 2 && !(bits(base) & 7) && !(pitch & 3)) return kLoraQuads;
+        return each == 2 && !(bits(base) & 3) ? kLoraWords : kLoraSingle;
+    };
+    p.how_a = how(a, cols, size, 16 / size), p.how_b = how(b, max_rank, size, per_b);
+    p.how_x = how(x, tokens == 1 ? 0 : x_stride, 4, 4), p.how_y = how(y, tokens == 1 ? 0 : y_stride, 4, 4);
+    const bool vec_a = p.how_a == kLoraWhole && p.how_x == kLoraWhole;
+    const bool vec_b = p.how_b == kLoraWhole && p.how_y == kLoraWhole && !(rows & 3);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool wide = tokens > kLoraScan;
     if (kind == 0) return wide ? lora_launch<float, 2>(p, vec_a, vec_b, s) : lora_launch<float, 1>(p, vec_a, vec_b, s);

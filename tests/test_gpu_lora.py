@@ -257,6 +257,19 @@ def test_few_tokens_in_one_launch_and_in_two(gpu_backend, kind, max_rank, cols, 
         Case(tokens, rows, cols, adapters, max_rank, kind, ids=ids, seed=tokens + cols).check(gpu_backend)
 
 
+@pytest.mark.parametrize('kind', [0, 1, 30])
+@pytest.mark.parametrize('offset', [0, 1, 2, 4])
+@pytest.mark.parametrize('max_rank,cols,rows', [(12, 1028, 64), (14, 1026, 66), (15, 257, 63), (36, 516, 68),
+                                                (37, 1025, 65), (60, 300, 4), (38, 10, 2), (3, 9, 1)])
+def test_rows_on_every_boundary(gpu_backend, kind, offset, max_rank, cols, rows):
+    """Rows that start on 8, 4 and 2 bytes, stacks that do not start on 4: what is read by the word stays inside the
+    stack (its last adapter's last row is used) and what it brings along does not count (NaN behind the ranks)."""
+    for tokens in (5, 70):
+        Case(tokens, rows, cols, 3, max_rank, kind, ids=np.arange(tokens) % 3, ranks=[max_rank - 2, 1, max_rank],
+             seed=tokens + cols).check(gpu_backend, offset=offset)
+    Case(40, rows, cols, 30, max_rank, kind, ids=np.arange(40) % 30, seed=cols).check(gpu_backend, offset=offset)
+
+
 @pytest.mark.parametrize('tokens,adapters,max_rank,cols,rows', [(1, 1, 16, 8192, 8192), (1, 1, 16, 8192, 8196),
                                                                 (9, 2, 64, 4096, 64), (9, 2, 64, 4088, 8)])
 def test_adapters_around_the_size_for_one_launch(gpu_backend, tokens, adapters, max_rank, cols, rows):
