@@ -629,7 +629,8 @@ struct LoraExpand {
                 for (int i = 0; i < 4; ++i) {
                     const int r = min(row + kLoraRows * q + i, VEC ? p.rows - 4 + i : p.rows - 1);
                     const W *from = b + static_cast<int64_t>(r) * p.max_rank + kChunk * c;
-                    // Behind the rank others' values may be read, up to the stack's end: the last chunk's mask drops them.
+                    // Behind the rank others' values may be read, up to the stack's end: the last chunk's mask drops
+                    // them.
                     int n = rank - kChunk * c - lane_r;
                     if (!VEC && n > 0) n = static_cast<int>(min(b_end - from, static_cast<ptrdiff_t>(16)));
                     if constexpr (KU == 2) {
