@@ -287,7 +287,11 @@ class BatchScheduler:
                 if r.rules and chosen[r.slot] < 0:
                     self._finish(r, 'exhausted', 'no token is allowed')
                     continue
-                token = self._sample(logits[r.slot], r) if r.temperature > 0 else int(chosen[r.slot])
+                try:
+                    token = self._sample(logits[r.slot], r) if r.temperature > 0 else int(chosen[r.slot])
+                except ValueError as exc:  # nothing to sample from: rules can sum up to an infinite logit
+                    self._finish(r, 'error', str(exc))
+                    continue
                 r.output.append(token)
                 r.generated += 1
                 r.next_token = token

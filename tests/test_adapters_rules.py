@@ -358,3 +358,18 @@ def test_submit_refusals(serve):
     with pytest.raises(ValueError, match='adapter'):
         plain.submit([1], 2, adapter=0)
     assert len(collect(plain.submit([1], 2, repetition_penalty=1, logit_bias={}))[0]) == 2
+
+
+@pytest.mark.parametrize('rules', [dict(frequency_penalty=-3e38, logit_bias={4: 3e38}),
+                                   dict(presence_penalty=-3e38, logit_bias={4: 3e38})])
+def test_a_request_whose_logits_overflow_ends_alone(serve, rules):
+    """Finite rules can sum up to an infinite logit, which cannot be sampled: that request ends, the others go on."""
+    sched = serve(2, 50)
+    sched.decoder.table[0, 4, 4] = 50.0  # 4 says 4, so that its penalties count
+    with np.errstate(over='ignore'):
+        fine = sched.submit([7, 8], 6)
+        tokens, done = collect(sched.submit([4], 6, temperature=1.0, **rules), timeout=5)
+        assert done['reason'] == 'error' and 'nonfinite' in done['error']
+        assert collect(fine, timeout=5)[0] == greedy(sched.decoder.table[0], 8, 6)
+        assert sched.thread.is_alive() and sched.status()['active_requests'] == 0
+        assert collect(sched.submit([7, 8], 6), timeout=5)[0] == greedy(sched.decoder.table[0], 8, 6)
