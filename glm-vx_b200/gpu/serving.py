@@ -201,6 +201,12 @@ class BatchScheduler:
         except queue.Full:
             pass
 
+    def _fail(self, exc, requests):
+        """Ends the requests that the decoder's failure `exc` leaves without a result."""
+        self.error = str(exc)
+        for req in requests:
+            self._finish(req, 'error', str(exc))
+
     def _sample(self, logits, req):
         logits = np.asarray(logits, dtype=np.float32)
         # a request's own rules may take tokens out (-inf); anything else that is not finite is an error
@@ -223,9 +229,9 @@ class BatchScheduler:
             free = self.slots.index(None)
             req.slot = free
             self.slots[free] = req
-            self.decoder.reset_slot(free)
-            self.slot_len[free] = 0
             try:
+                self.decoder.reset_slot(free)
+                self.slot_len[free] = 0
                 if getattr(self.decoder, 'adapters', None) is not None:
                     self.decoder.set_adapter(free, req.adapter)
                 if req.rules:
@@ -233,10 +239,15 @@ class BatchScheduler:
                     self.decoder.rules.set(free, prompt=len(req.tokens), allowed=fixed, **req.rules)
             except ValueError as exc:  # the adapter was unloaded meanwhile, or the like: this request's own failure
                 self._finish(req, 'error', str(exc))
+            except Exception as exc:  # the device's, which the other requests meet in their next step
+                self._fail(exc, [req])
         for b, r in enumerate(self.slots):
             if r is None and self.slot_len[b] >= self.decoder.capacity - 1:
-                self.decoder.reset_slot(b)
-                self.slot_len[b] = 0
+                try:
+                    self.decoder.reset_slot(b)
+                    self.slot_len[b] = 0
+                except Exception as exc:  # its cache would run over in a step of the others
+                    self._fail(exc, [r for r in self.slots if r is not None])
         return closed
 
     def _run(self):
@@ -274,9 +285,7 @@ class BatchScheduler:
                 self.steps += 1
                 self.slot_len = [n + 1 for n in self.slot_len]
             except Exception as exc:  # the device or a bounded wait failed: every active request ends
-                self.error = str(exc)
-                for r in active:
-                    self._finish(r, 'error', str(exc))
+                self._fail(exc, active)
                 continue
             for r in active:
                 r.decode_seconds += dt

@@ -373,3 +373,41 @@ def test_a_request_whose_logits_overflow_ends_alone(serve, rules):
         assert collect(fine, timeout=5)[0] == greedy(sched.decoder.table[0], 8, 6)
         assert sched.thread.is_alive() and sched.status()['active_requests'] == 0
         assert collect(sched.submit([7, 8], 6), timeout=5)[0] == greedy(sched.decoder.table[0], 8, 6)
+
+
+def test_a_failing_admission_ends_its_request_alone(serve):
+    """What the device or the decoder raises while a request is put into its slot ends that request."""
+    from gpu.runtime import CUDAError
+    sched = serve(2, 50)
+    clear = sched.decoder.rules.clear
+
+    def fails(b):
+        raise CUDAError('glmvx_stream_synchronize', 700, 'as if')
+
+    sched.decoder.rules.clear = fails
+    tokens, done = collect(sched.submit([4], 3), timeout=5)
+    assert tokens == [] and done['reason'] == 'error' and 'as if' in done['error']
+    assert sched.thread.is_alive() and sched.status()['active_requests'] == 0 and 'as if' in sched.status()['error']
+    sched.decoder.rules.clear = clear
+    assert collect(sched.submit([4], 3), timeout=5)[0] == greedy(sched.decoder.table[0], 4, 3)
+
+
+def test_a_failing_reset_of_an_idle_slot_ends_what_runs(serve):
+    """An idle slot is emptied before its cache is full; where that fails, the requests of the step end with the
+    device's error, and the worker stays."""
+    from gpu.runtime import CUDAError
+    sched = serve(2, 50)
+    reset, failed = sched.decoder.reset_slot, []
+
+    def fails(b):
+        if b == 1:
+            failed.append(b)
+            raise CUDAError('glmvx_memset', 700, 'as if')
+        reset(b)
+
+    sched.decoder.reset_slot = fails
+    for _ in range(2):  # slot 1 stays idle for more steps than a sequence has room for
+        tokens, done = collect(sched.submit([4], 40), timeout=5)
+    assert failed and done['reason'] == 'error' and 'as if' in done['error'] and len(tokens) < 40
+    sched.decoder.reset_slot = reset
+    assert collect(sched.submit([4], 3), timeout=5)[0] == greedy(sched.decoder.table[0], 4, 3)
