@@ -18,20 +18,25 @@ from . import runtime as rt
 MAX_BIAS = 2047
 
 
-def pack_mask(allowed, vocab):
-    """uint32 words, bit v % 32 of word v // 32 set where token v is allowed:
-    from a boolean array [vocab], or an array or iterable of token ids."""
-    words = (vocab + 31) // 32
+def allowed_tokens(allowed, vocab):
+    """A new boolean array [vocab], True where token v is allowed: from such an
+    array, or an array or iterable of token ids."""
     allowed = np.asarray(allowed if isinstance(allowed, np.ndarray) else list(allowed))
     if allowed.dtype == np.bool_:
         if allowed.shape != (vocab,):
             raise ValueError(f'a mask has one truth value for each of {vocab} tokens')
-        keep = allowed
-    else:
-        if allowed.size and (allowed.dtype.kind not in 'iu' or allowed.min() < 0 or allowed.max() >= vocab):
-            raise ValueError('allowed token ids must be in the vocabulary')
-        keep = np.zeros(vocab, bool)
-        keep[allowed.astype(np.int64).reshape(-1)] = True
+        return allowed.copy()
+    if allowed.size and (allowed.dtype.kind not in 'iu' or allowed.min() < 0 or allowed.max() >= vocab):
+        raise ValueError('allowed token ids must be in the vocabulary')
+    keep = np.zeros(vocab, bool)
+    keep[allowed.astype(np.int64).reshape(-1)] = True
+    return keep
+
+
+def pack_mask(allowed, vocab):
+    """uint32 words, bit v % 32 of word v // 32 set where token v is allowed
+    (`allowed` as in allowed_tokens)."""
+    words, keep = (vocab + 31) // 32, allowed_tokens(allowed, vocab)
     return np.packbits(np.pad(keep, (0, 32 * words - vocab)), bitorder='little').view('<u4').astype(np.uint32)
 
 
@@ -89,7 +94,8 @@ class LogitRules:
         prompt (they count for the repetition penalty only); tokens seen are
         divided (positive logits) or multiplied by `repetition`, output tokens
         lose `frequency` per occurrence and `presence` once; `bias` {token:
-        value} is added (-inf bans); `allowed` as in pack_mask (None: all)."""
+        value} is added (-inf bans); `allowed` as in allowed_tokens (None:
+        all)."""
         self._sequence(b)
         values = np.array([repetition, presence, frequency], np.float32)
         if not np.isfinite(values).all() or repetition <= 0 or values[0] <= 0:

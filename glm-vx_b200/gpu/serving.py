@@ -37,7 +37,7 @@ import uuid
 
 import numpy as np
 
-from .rules import pack_mask
+from .rules import allowed_tokens
 
 
 class BusyError(Exception):
@@ -98,8 +98,9 @@ class BatchScheduler:
                presence_penalty=0.0, frequency_penalty=0.0, logit_bias=None, allowed=None):
         """adapter: a loaded slot of the decoder's bank.  logit_bias: {token:
         value to add, -inf to ban}.  allowed: the tokens that may be said, as a
-        boolean array over the vocabulary or token ids, or a function from
-        the list of tokens generated so far to such a mask (or None: all)."""
+        boolean array over the vocabulary or token ids (copied here), or a
+        function from the list of tokens generated so far to such a mask (or
+        None: all)."""
         cfg = self.config
         if not isinstance(tokens, list) or not tokens or any(type(t) is not int or not 0 <= t < cfg['vocab_size']
                                                              for t in tokens):
@@ -111,7 +112,7 @@ class BatchScheduler:
             raise ValueError('temperature must be finite and nonnegative')
         if type(seed) is not int or seed < 0:
             raise ValueError('seed must be a nonnegative integer')
-        rules = self._rules(repetition_penalty, presence_penalty, frequency_penalty, logit_bias, allowed)
+        rules, allowed = self._rules(repetition_penalty, presence_penalty, frequency_penalty, logit_bias, allowed)
         if adapter is not None:
             bank = getattr(self.decoder, 'adapters', None)
             if bank is None or type(adapter) is not int or not 0 <= adapter < bank.slots or not bank.loaded[adapter]:
@@ -136,7 +137,9 @@ class BatchScheduler:
         return req
 
     def _rules(self, repetition, presence, frequency, bias, allowed):
-        """The request's rules as LogitRules.set takes them ({}: none)."""
+        """The request's rules as LogitRules.set takes them ({}: none), and
+        `allowed` as a mask of its own (an iterable is read once, an array may
+        change) or the function that it is."""
         rules = getattr(self.decoder, 'rules', None)
         numbers = {'repetition_penalty': repetition, 'presence_penalty': presence, 'frequency_penalty': frequency}
         for name, value in numbers.items():
@@ -153,15 +156,15 @@ class BatchScheduler:
                     np.float32(value) == np.inf:
                 raise ValueError('logit_bias values must be finite or -inf')
         if (repetition, presence, frequency) == (1.0, 0.0, 0.0) and not bias and allowed is None:
-            return {}
+            return {}, None
         if rules is None:
             raise ValueError('the decoder has no logit rules')
         if len(bias) > rules.max_bias:
             raise ValueError(f'logit_bias names more than {rules.max_bias} tokens')
         if allowed is not None and not callable(allowed):
-            pack_mask(allowed, vocab)  # its ValueErrors now, not in the worker
+            allowed = allowed_tokens(allowed, vocab)
         return {'repetition': float(repetition), 'presence': float(presence), 'frequency': float(frequency),
-                'bias': bias}
+                'bias': bias}, allowed
 
     def cancel(self, req):
         req.cancelled.set()

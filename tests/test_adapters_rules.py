@@ -411,3 +411,29 @@ def test_a_failing_reset_of_an_idle_slot_ends_what_runs(serve):
     assert failed and done['reason'] == 'error' and 'as if' in done['error'] and len(tokens) < 40
     sched.decoder.reset_slot = reset
     assert collect(sched.submit([4], 3), timeout=5)[0] == greedy(sched.decoder.table[0], 4, 3)
+
+
+@pytest.mark.parametrize('allowed', [lambda: iter([3, 4]), lambda: (t for t in [3, 4]), lambda: map(int, '34'),
+                                     lambda: {3: 'x', 4: 'y'}.keys()])
+def test_allowed_tokens_that_can_be_read_once(serve, allowed):
+    sched = serve(2, 50)
+    tokens, done = collect(sched.submit([7], 4, allowed=allowed()))
+    assert len(tokens) == 4 and set(tokens) <= {3, 4} and done['reason'] == 'length'
+
+
+@pytest.mark.parametrize('boolean', [False, True])
+def test_a_mask_is_the_one_that_was_submitted(serve, boolean):
+    """What the caller does to its array or list after submit() counts for nothing."""
+    sched = serve(2, 50)
+    mask = [3, 4]
+    if boolean:
+        mask = np.zeros(50, bool)
+        mask[[3, 4]] = True
+    with sched.lock:  # the worker admits after this block
+        req = sched.submit([7], 4, allowed=mask)
+        if boolean:
+            mask[:] = False
+            mask[9] = True
+        else:
+            mask[:] = [9]
+    assert set(collect(req)[0]) <= {3, 4}
