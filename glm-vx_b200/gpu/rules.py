@@ -11,11 +11,22 @@ needs no new capture and no logits on the host.
 The reference takes the model's logits as they are (glm_vx/generate.py:96,
 glm_vx/scheduler.py:113-120); this has no counterpart there.
 """
+import operator
+
 import numpy as np
 
 from . import runtime as rt
 
 MAX_BIAS = 2047
+
+
+def to_f32(value):
+    """The value as a float32, infinite beyond its range (whole numbers too)."""
+    with np.errstate(over='ignore'):
+        try:
+            return np.float32(value)
+        except OverflowError:
+            return np.float32(np.inf if value > 0 else -np.inf)
 
 
 def allowed_tokens(allowed, vocab):
@@ -97,24 +108,27 @@ class LogitRules:
         value} is added (-inf bans); `allowed` as in allowed_tokens (None:
         all)."""
         self._sequence(b)
-        values = np.array([repetition, presence, frequency], np.float32)
-        if not np.isfinite(values).all() or repetition <= 0 or values[0] <= 0:
+        values = np.array([to_f32(v) for v in (repetition, presence, frequency)])
+        if not np.isfinite(values).all() or values[0] <= 0:
             raise ValueError('penalties must be finite, the repetition penalty positive')
         if int(prompt) < 0:
             raise ValueError('prompt length must be nonnegative')
-        bias = dict(bias or {})
+        try:
+            bias = {operator.index(t): to_f32(v) for t, v in dict(bias or {}).items()}
+        except TypeError as exc:
+            raise ValueError('biased tokens must be whole numbers') from exc
         if len(bias) > self.max_bias:
             raise ValueError(f'more than {self.max_bias} biased tokens')
-        if any(not 0 <= int(t) < self.vocab for t in bias):
+        if any(not 0 <= t < self.vocab for t in bias):
             raise ValueError('biased tokens must be in the vocabulary')
         biases = np.array(list(bias.values()), np.float32)
         if np.isnan(biases).any() or (biases == np.inf).any():
             raise ValueError('biases must be finite or -inf')
         words = None if allowed is None else pack_mask(allowed, self.vocab)
-        self._put('prompts', np.array([prompt], np.int32), b)
+        self._put('prompts', np.array([min(int(prompt), 2**31 - 1)], np.int32), b)
         self._put('penalties', values, b, 3)
         if bias:
-            self._put('bias_ids', np.array([int(t) for t in bias], np.int32), b, self.max_bias)
+            self._put('bias_ids', np.array(list(bias), np.int32), b, self.max_bias)
             self._put('bias_values', biases, b, self.max_bias)
         self._put('bias_lens', np.array([len(bias)], np.int32), b)
         self._mask(b, words)

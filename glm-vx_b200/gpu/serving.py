@@ -31,13 +31,14 @@ applied on the device; a request whose rules leave no token ends with reason
 from collections import deque
 from dataclasses import dataclass, field
 import queue
+import sys
 import threading
 import time
 import uuid
 
 import numpy as np
 
-from .rules import allowed_tokens
+from .rules import allowed_tokens, to_f32
 
 
 class BusyError(Exception):
@@ -108,7 +109,7 @@ class BatchScheduler:
         if type(max_tokens) is not int or max_tokens < 1:
             raise ValueError('max_tokens must be a positive integer')
         if not isinstance(temperature, (int, float)) or isinstance(temperature, bool) or \
-                not np.isfinite(temperature) or temperature < 0:
+                not 0 <= temperature <= sys.float_info.max:
             raise ValueError('temperature must be finite and nonnegative')
         if type(seed) is not int or seed < 0:
             raise ValueError('seed must be a nonnegative integer')
@@ -143,17 +144,16 @@ class BatchScheduler:
         rules = getattr(self.decoder, 'rules', None)
         numbers = {'repetition_penalty': repetition, 'presence_penalty': presence, 'frequency_penalty': frequency}
         for name, value in numbers.items():
-            if not isinstance(value, (int, float)) or isinstance(value, bool) or not np.isfinite(np.float32(value)):
+            if not isinstance(value, (int, float)) or isinstance(value, bool) or not np.isfinite(to_f32(value)):
                 raise ValueError(f'{name} must be finite')
-        if not np.float32(repetition) > 0:
+        if not to_f32(repetition) > 0:
             raise ValueError('repetition_penalty must be positive')
         bias = dict(bias or {})
         vocab = self.config['vocab_size']
         for token, value in bias.items():
             if type(token) is not int or not 0 <= token < vocab:
                 raise ValueError('logit_bias must name valid token IDs')
-            if not isinstance(value, (int, float)) or isinstance(value, bool) or np.isnan(value) or \
-                    np.float32(value) == np.inf:
+            if not isinstance(value, (int, float)) or isinstance(value, bool) or not to_f32(value) < np.inf:
                 raise ValueError('logit_bias values must be finite or -inf')
         if (repetition, presence, frequency) == (1.0, 0.0, 0.0) and not bias and allowed is None:
             return {}, None
@@ -164,7 +164,7 @@ class BatchScheduler:
         if allowed is not None and not callable(allowed):
             allowed = allowed_tokens(allowed, vocab)
         return {'repetition': float(repetition), 'presence': float(presence), 'frequency': float(frequency),
-                'bias': bias}, allowed
+                'bias': {token: float(to_f32(value)) for token, value in bias.items()}}, allowed
 
     def cancel(self, req):
         req.cancelled.set()

@@ -437,3 +437,43 @@ def test_a_mask_is_the_one_that_was_submitted(serve, boolean):
         else:
             mask[:] = [9]
     assert set(collect(req)[0]) <= {3, 4}
+
+
+def test_numbers_beyond_every_range(serve):
+    """Whole numbers that no float holds are refused, or stand for a ban, as floats beyond float32 do."""
+    sched = serve(1, 50)
+    big = 10 ** 400
+    for change in (dict(repetition_penalty=big), dict(presence_penalty=-big), dict(frequency_penalty=big),
+                   dict(logit_bias={1: big}), dict(logit_bias={1: 1e39}), dict(temperature=big)):
+        with pytest.raises(ValueError):
+            sched.submit([1], 2, **change)
+    first = greedy(sched.decoder.table[0], 4, 1)[0]
+    for ban in (-big, -1e39, float('-inf')):
+        tokens, done = collect(sched.submit([4], 1, logit_bias={first: ban}))
+        assert done['reason'] == 'length' and tokens != [first]
+
+
+@pytest.mark.parametrize('change,message', [
+    (dict(repetition=10 ** 400), 'finite'), (dict(presence=-10 ** 400), 'finite'), (dict(frequency=1e39), 'finite'),
+    (dict(bias={3: 10 ** 400}), 'biases'), (dict(bias={3: float('nan')}), 'biases'), (dict(prompt=-1), 'prompt'),
+    (dict(bias={1.5: 1.0}), 'biased tokens'), (dict(bias={'1': 1.0}), 'biased tokens'),
+    (dict(bias={50: 1.0}), 'biased tokens'), (dict(bias={-1: 1.0}), 'biased tokens'),
+    (dict(bias={i: 0.0 for i in range(5)}), 'more than 4'), (dict(repetition=0.0), 'positive')])
+def test_rules_that_cannot_be_set(change, message):
+    backend = QuietBackend()
+    rules = LogitRules.__new__(LogitRules)
+    rules.backend, rules.batch, rules.vocab, rules.max_bias, rules._bufs = backend, 2, 50, 4, {}
+    with pytest.raises(ValueError, match=message):
+        rules.set(1, **change)
+    assert not backend.held  # nothing was put into place
+
+
+def test_a_prompt_longer_than_any_history():
+    """All that is fed is prompt, as with any prompt that is not yet at its end."""
+    backend, put = QuietBackend(), {}
+    rules = LogitRules.__new__(LogitRules)
+    rules.backend, rules.batch, rules.vocab, rules.max_bias, rules._masked = backend, 2, 50, 4, [False, False]
+    rules._put = lambda name, array, item, width=1: put.__setitem__(name, np.array(array))
+    rules.set(1, prompt=10 ** 12, bias={np.int64(7): -10 ** 400})
+    assert put['prompts'].tolist() == [2 ** 31 - 1] and put['prompts'].dtype == np.int32
+    assert put['bias_ids'].tolist() == [7] and put['bias_values'].tolist() == [-np.inf]
