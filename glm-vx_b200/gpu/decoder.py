@@ -122,7 +122,7 @@ class ResidentDecoder:
     are added to this model's, each sequence by the adapter that set_adapter
     gave it (none at first).  The bank stays the caller's to close.
     rules (optional): a LogitRules (gpu/rules.py) of this batch and
-    vocabulary; a step's logits are then the ones its rules leave, and the
+    vocabulary, with histories as long as the sequences; a step's logits are then the ones its rules leave, and the
     chosen token is -1 where they leave nothing."""
 
     def __init__(self, backend, config, source, batch, capacity, layers=None, moe_layer_factory=None, adapters=None,
@@ -155,6 +155,8 @@ class ResidentDecoder:
         if rules is not None and (rules.batch, rules.vocab) != (self.B, self.vocab):
             raise ValueError(f'rules are for {rules.batch} sequences over {rules.vocab} tokens, '
                              f'not {self.B} over {self.vocab}')
+        if rules is not None and rules.capacity < self.capacity:  # what is fed after that would count for nothing
+            raise ValueError(f'the rules\' histories hold {rules.capacity} tokens, the sequences {self.capacity}')
         if adapters is not None:
             shapes = projection_shapes(c, self.n_layers)
             for name, shape in adapters.shapes.items():

@@ -477,3 +477,16 @@ def test_a_prompt_longer_than_any_history():
     rules.set(1, prompt=10 ** 12, bias={np.int64(7): -10 ** 400})
     assert put['prompts'].tolist() == [2 ** 31 - 1] and put['prompts'].dtype == np.int32
     assert put['bias_ids'].tolist() == [7] and put['bias_values'].tolist() == [-np.inf]
+
+
+@pytest.mark.parametrize('remembered,refused', [(7, True), (8, False), (9, False)])
+def test_rules_remember_as_much_as_a_sequence_holds(remembered, refused):
+    """Past its capacity a history stops growing and the penalties no longer follow the output: a decoder whose
+    sequences are longer than that is refused."""
+    from gpu.decoder import ResidentDecoder
+    config = dict(CONFIG, index_n_heads=2, index_head_dim=16, index_topk=8, indexer_types=['full', 'full'])
+    backend = NoDevice()
+    rules = SimpleNamespace(backend=backend, batch=2, vocab=50, capacity=remembered)
+    with pytest.raises(ValueError if refused else Exception) as raised:
+        ResidentDecoder(backend, config, None, batch=2, capacity=8, rules=rules)
+    assert ('histories' in str(raised.value)) == refused
