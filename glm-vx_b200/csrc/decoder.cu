@@ -5,7 +5,8 @@
 // step is one replayable graph).
 //
 //   embed_rows      x[b] = row ids[b] of the embedding table (F32, or Q8_0
-//                   decoded exactly: fp16 d times int8 q), model.py:96-104
+//                   decoded exactly: fp16 d times int8 q), model.py:96-104;
+//                   -1 (a sequence at its end, glmvx_logits_select) takes row 0
 //   rope_rows       the reference's rope (kernels/kernels.vx:425-441: pairs
 //                   (x[2p], x[2p+1]) rotated, output half-split) on strided
 //                   rows at each sequence's position, with the cos/sin taken
@@ -40,7 +41,7 @@ __global__ void embed_rows_kernel(float *out, const uint8_t *table, int kind, co
     const int b = blockIdx.x;
     int id = ids[b];
     if (id < 0 || id >= vocab) {
-        if (threadIdx.x == 0) report_device_error(err, kDevErrBadIndex);
+        if (id != -1 && threadIdx.x == 0) report_device_error(err, kDevErrBadIndex);
         id = min(max(id, 0), vocab - 1);
     }
     float *o = out + static_cast<size_t>(b) * hidden;

@@ -122,8 +122,9 @@ class ResidentDecoder:
     are added to this model's, each sequence by the adapter that set_adapter
     gave it (none at first).  The bank stays the caller's to close.
     rules (optional): a LogitRules (gpu/rules.py) of this batch and
-    vocabulary, with histories as long as the sequences; a step's logits are then the ones its rules leave, and the
-    chosen token is -1 where they leave nothing."""
+    vocabulary, with histories as long as the sequences; a step's logits are
+    then the ones its rules leave, and the chosen token is -1 where they leave
+    nothing (fed again, it embeds row 0 and joins no history)."""
 
     def __init__(self, backend, config, source, batch, capacity, layers=None, moe_layer_factory=None, adapters=None,
                  rules=None):
@@ -525,7 +526,9 @@ class ResidentDecoder:
     def generate(self, prompts, new_tokens, with_logits=False):
         """Greedy decode (glm_vx/generate.py:86-109 for each sequence):
         prompts [B][P] token ids, every sequence from an empty cache; returns
-        (generated [B][new_tokens], logits of every sampled step or None)."""
+        (generated [B][new_tokens], logits of every sampled step or None).  A
+        sequence whose rules leave it nothing has -1 from then on; the others
+        go on."""
         prompts = np.asarray(prompts, np.int64)
         if prompts.shape[0] != self.B or prompts.ndim != 2 or prompts.shape[1] < 1:
             raise ValueError('prompts must be [batch, length >= 1]')
@@ -537,7 +540,8 @@ class ResidentDecoder:
         for i in range(new_tokens):
             if with_logits:
                 logits.append(self.read_logits())
-            out.append(self.read_tokens())
+            chosen = self.read_tokens()
+            out.append(np.where(out[-1] < 0, -1, chosen) if out else chosen)
             if i + 1 < new_tokens:
                 self.step()
         self.check()

@@ -343,7 +343,10 @@ int32_t glmvx_ep_destroy(void *layer);
 /* Batched decode-step pieces of the GLM-MoE-DSA model (one token for each of
  * `tokens` sequences, device pointers; the reference runs them per token on
  * the host, glm_vx/model.py:96-237, 359-392).
- *   glmvx_embed_rows   x[b] = row ids[b] of an F32 (kind 0) or Q8_0 (8) table
+ *   glmvx_embed_rows   x[b] = row ids[b] of an F32 (kind 0) or Q8_0 (8) table;
+ *                      -1, which glmvx_logits_select leaves a sequence that has
+ *                      nothing to say, takes row 0, any other id outside the
+ *                      table the nearest and sets the device error word (3)
  *   glmvx_rope_rows    the reference rope (kernels/kernels.vx:425-441, pairs
  *                      rotated, output half-split) of `d` elements of `heads`
  *                      strided rows per sequence at position pos[b], cos/sin

@@ -490,3 +490,15 @@ def test_rules_remember_as_much_as_a_sequence_holds(remembered, refused):
     with pytest.raises(ValueError if refused else Exception) as raised:
         ResidentDecoder(backend, config, None, batch=2, capacity=8, rules=rules)
     assert ('histories' in str(raised.value)) == refused
+
+
+def test_a_sequence_that_nothing_is_left_to_stays_at_its_end():
+    """generate() goes on with the others; the ended row keeps -1 whatever its later steps would choose."""
+    from gpu.decoder import ResidentDecoder
+    dec = ResidentDecoder.__new__(ResidentDecoder)
+    dec.B, steps, choices = 3, [], [[5, 6, 7], [5, -1, 8], [-1, 3, 9], [4, -1, 2]]
+    dec.reset = dec.check = lambda: None
+    dec.set_tokens, dec.step = lambda tokens: None, lambda: steps.append('step')
+    dec.read_tokens = lambda: np.array(choices[steps.count('step') - 1], np.int32)
+    out, _ = dec.generate([[1], [2], [3]], 4)
+    assert out.tolist() == [[5, 5, -1, -1], [6, -1, -1, -1], [7, 8, 9, 2]]

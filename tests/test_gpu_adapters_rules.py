@@ -308,3 +308,28 @@ def test_scheduler_serves_different_users_at_once(gpu_backend):
         dec.close()
         rules.close()
         bank.close()
+
+
+def test_generate_with_a_sequence_that_nothing_is_left_to(gpu_backend):
+    """The ended row returns -1 from then on, nothing is reported and the other rows say what they say without rules."""
+    from gpu.rules import LogitRules
+    plain = decoder(gpu_backend)
+    rules = LogitRules(gpu_backend, len(PROMPTS), CONFIG['vocab_size'], capacity=40)
+    dec = decoder(gpu_backend, rules=rules)
+    try:
+        want, logits = plain.generate(PROMPTS, 6, with_logits=True)
+        rules.set(1, allowed=[])
+        got, seen = dec.generate(PROMPTS, 6, with_logits=True)
+        assert got[1].tolist() == [-1] * 6 and (seen[1] == -np.inf).all()
+        assert np.array_equal(got[[0, 2]], want[[0, 2]])
+        assert seen[[0, 2]].tobytes() == logits[[0, 2]].tobytes()
+        rules.set(1, prompt=4, frequency=3e38, allowed=[7])  # twice 3e38 is infinite: 7 may be said two times
+        got, _ = dec.generate(PROMPTS, 6)
+        assert got[1].tolist() == [7, 7, -1, -1, -1, -1]
+        assert np.array_equal(got[[0, 2]], want[[0, 2]])
+        rules.set(1)
+        assert np.array_equal(dec.generate(PROMPTS, 6)[0], want)
+    finally:
+        dec.close()
+        plain.close()
+        rules.close()
