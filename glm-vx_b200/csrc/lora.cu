@@ -867,8 +867,13 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_cluster_kernel(LoraArgs 
 
 constexpr int lora_ceil(int64_t n, int64_t of) { return static_cast<int>((n + of - 1) / of); }
 
-// Parts that the columns are cut into, at most: enough CTAs for few tokens.
-int lora_max_splits(int tokens) { return std::clamp(lora_ceil(16384, tokens), 1, kLoraMaxSplits); }
+// Parts that the columns are cut into, at most: enough CTAs for few tokens, and at most so many parts of h in all
+// (or one a token), a bound that fewer tokens do not pass: a workspace does for fewer tokens too.
+constexpr int kLoraMaxParts = 16384;
+int lora_max_splits(int tokens) { return std::clamp(kLoraMaxParts / tokens, 1, kLoraMaxSplits); }
+int64_t lora_max_parts(int64_t tokens) {
+    return std::min<int64_t>(kLoraMaxSplits * tokens, std::max<int64_t>(kLoraMaxParts, tokens));
+}
 
 // Tiles of `size` tokens there may be: each but an adapter's last one is full.
 int64_t lora_most_tiles(int64_t tokens, int64_t adapters, int size) {
@@ -887,7 +892,7 @@ LoraLayout lora_layout(int64_t tokens, int64_t adapters, int64_t max_rank) {
         l.bytes += (n + 15) & ~int64_t{15};
         return at;
     };
-    take(4 * tokens * lora_h_pitch(static_cast<int>(max_rank)) * lora_max_splits(static_cast<int>(tokens)));
+    take(4 * lora_max_parts(tokens) * lora_h_pitch(static_cast<int>(max_rank)));
     if (tokens > kLoraScan) {
         l.tiles = take(sizeof(LoraTile) * lora_most_tiles(tokens, adapters, kLoraTile));
         l.places = take(4 * tokens);

@@ -398,8 +398,9 @@ int32_t glmvx_dsa_attend(float *out, const int32_t *selected, const float *q_lat
  * does not depend on the other tokens' adapters and is the same every time.
  * tokens <= 2^20, rows and cols <= 2^22, adapters <= 2^24, max_rank <= 256.
  * y must not overlap x.  Pointers belong to the current device.  workspace:
- * device scratch of glmvx_lora_workspace_bytes(...) bytes, 16-byte aligned; calls
- * that may overlap in time need one each. */
+ * device scratch of glmvx_lora_workspace_bytes(...) bytes (no less for more
+ * tokens, adapters or ranks: one does for all smaller calls), 16-byte aligned;
+ * calls that may overlap in time need one each. */
 int64_t glmvx_lora_workspace_bytes(int32_t tokens, int32_t adapters, int32_t max_rank);
 int32_t glmvx_lora_add(float *y, int64_t y_stride, const float *x, int64_t x_stride, const int32_t *adapter_ids,
                        int32_t kind, const void *a, const void *b, const int32_t *ranks, const float *scales,

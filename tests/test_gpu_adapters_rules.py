@@ -333,3 +333,42 @@ def test_generate_with_a_sequence_that_nothing_is_left_to(gpu_backend):
         dec.close()
         plain.close()
         rules.close()
+
+
+@pytest.mark.parametrize('max_tokens', [600, 4096])
+def test_a_bank_of_prompts_takes_every_number_of_tokens(gpu_backend, max_tokens):
+    """One workspace, made for the most tokens, holds fewer ones' call.  Against 64 bits: a sum of K products is off by
+    (K / 8 + 40) * 2^-23 + 3 * 2^-22 of its absolute terms at most (test_gpu_lora.py says why), which is 29 * 2^-22 for
+    96 and 24 * 2^-22 for 8: 64 * 2^-22 holds both and what they make of one another."""
+    from gpu import runtime as rt
+    from gpu.adapters import AdapterBank
+    rng = np.random.default_rng(max_tokens)
+    rows, cols, rank, slots = 40, 96, 8, 16
+    bank = AdapterBank(gpu_backend, {'p': (rows, cols)}, slots, rank, kind=0, max_tokens=max_tokens)
+    weights = [(rng.normal(size=(rank, cols)).astype(np.float32), rng.normal(size=(rows, rank)).astype(np.float32))
+               for _ in range(slots)]
+    for i, pair in enumerate(weights):
+        bank.load(i, {'p': pair}, 0.5)
+    x, y = rng.normal(size=(max_tokens, cols)).astype(np.float32), np.zeros((max_tokens, rows), np.float32)
+    ids = rng.integers(-1, slots, max_tokens).astype(np.int32)
+    bufs = [rt.DeviceBuffer(v.nbytes) for v in (y, x, ids)]
+    want, mass = np.zeros((max_tokens, rows)), np.zeros((max_tokens, rows))
+    for i, (a, b) in enumerate(weights):
+        mine = ids == i
+        want[mine] = 0.5 * (x[mine].astype(np.float64) @ a.T.astype(np.float64)) @ b.T.astype(np.float64)
+        mass[mine] = 0.5 * (np.abs(x[mine]) @ np.abs(a.T)) @ np.abs(b.T)
+    try:
+        for buf, v in zip(bufs, (y, x, ids)):
+            buf.upload(v, gpu_backend.stream.handle)
+        for tokens in sorted({1, 64, 65, 100, max_tokens // 2 + 1, max_tokens - 96, max_tokens - 1, max_tokens}):
+            bufs[0].upload(y, gpu_backend.stream.handle)
+            bank.add('p', *(buf.ptr for buf in bufs), tokens)
+            got = np.empty_like(y)
+            bufs[0].download(got, gpu_backend.stream.handle)
+            gpu_backend.stream.synchronize()
+            assert (np.abs(got[:tokens] - want[:tokens]) <= 64 * 2.0 ** -22 * mass[:tokens]).all()
+            assert not got[tokens:].any()
+    finally:
+        for buf in bufs:
+            buf.close()
+        bank.close()

@@ -40,3 +40,13 @@ def test_workspace_size():
     assert size(64, 4, 16) >= 64 * 16 * 4
     for bad in ((-1, 1, 1), ((1 << 20) + 1, 1, 1), (1, 0, 1), (1, (1 << 24) + 1, 1), (1, 1, 0), (1, 1, 257)):
         assert size(*bad) < 0
+
+
+@pytest.mark.parametrize('adapters,max_rank', [(1, 1), (16, 32), (24, 64), (4, 16), (300, 256)])
+def test_a_workspace_does_for_fewer_tokens_too(adapters, max_rank):
+    """A bank asks once, for the most tokens it takes."""
+    size = rt.library().glmvx_lora_workspace_bytes
+    need = [size(t, adapters, max_rank) for t in [*range(1, 20000), *range(20000, 1 << 20, 4097), 1 << 20]]
+    assert all(a <= b for a, b in zip(need, need[1:]))
+    # h holds at least a part of every token
+    assert need[-1] >= 4 * max_rank << 20
