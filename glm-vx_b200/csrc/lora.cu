@@ -195,14 +195,26 @@ __device__ __forceinline__ uint32_t lora_tf32(float x) {
     return r;
 }
 
-// x = hi + lo, both TF32.
+// The same, and the largest TF32 number of the sign where that is beyond it.
+__device__ __forceinline__ uint32_t lora_tf32_within(float x) {
+    uint32_t r;
+    asm("cvt.rna.satfinite.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
+    return r;
+}
+
+// x = hi + lo, both TF32.  Of an infinite x (and of one that hi rounds up to infinity) lo is not a number, but with
+// WIDE: infinity is then the largest number and infinity, whose products with a weight have one sign.
+template <bool WIDE>
+__device__ __forceinline__ void lora_split(float x, uint32_t &hi, uint32_t &lo) {
+    hi = WIDE ? lora_tf32_within(x) : lora_tf32(x);
+    lo = lora_tf32(x - __uint_as_float(hi));
+}
+
+template <bool WIDE>
 __device__ __forceinline__ void lora_split(const float4 &x, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
     const float v[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        hi[e] = lora_tf32(v[e]);
-        lo[e] = lora_tf32(v[e] - __uint_as_float(hi[e]));
-    }
+    for (int e = 0; e < 4; ++e) lora_split<WIDE>(v[e], hi[e], lo[e]);
 }
 
 __device__ __forceinline__ void lora_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -221,8 +233,8 @@ __device__ __forceinline__ void lora_unit(float (&c)[4], const float4 &top, cons
     uint32_t th[4], lh[4];
     if constexpr (SPLIT) {
         uint32_t tl[4], ll[4];
-        lora_split(top, th, tl);
-        lora_split(low, lh, ll);
+        lora_split<false>(top, th, tl);
+        lora_split<false>(low, lh, ll);
 #pragma unroll
         for (int s = 0; s < 4; s += 2) lora_mma(c, tl[s], ll[s], tl[s + 1], ll[s + 1], hi[s], hi[s + 1]);
     } else {
@@ -391,6 +403,25 @@ __global__ void __launch_bounds__(kLoraPlanThreads) lora_plan_kernel(LoraArgs p)
     if (tid == 0) *p.ntiles = base;
 }
 
+__device__ __forceinline__ float lora_value(float w) { return w; }
+__device__ __forceinline__ float lora_value(__half w) { return __half2float(w); }
+__device__ __forceinline__ float lora_value(__nv_bfloat16 w) { return __bfloat162float(w); }
+
+// w . x over n columns in plain f32, sixteen sums side by side; ends with the first that is not a number.
+template <class W>
+__device__ __noinline__ float lora_plain(const W *w, const float *x, int n) {
+    float v[16] = {}, sum = 0.0f;
+    for (int c = 0; c < n && sum == sum; c += 16) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+            if (c + k < n) v[k] = fmaf(lora_value(w[c + k]), x[c + k], v[k]);
+        sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) sum += v[k];
+    }
+    return sum;
+}
+
 // A . x for a tile of 8 NT tokens, 16 MT MW ranks and a range of columns, by one
 // CTA.  MW warps share a block of 32 columns, 16 MT ranks each, and take every
 // 8 / MW-th block, the next one on its way meanwhile; the warps' sums are joined
@@ -438,7 +469,7 @@ struct LoraShrink {
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
                     uint32_t hi[4], lo[4];
-                    lora_split(lora_f32<float>(t.x[j].q[k]), hi, lo);
+                    lora_split<false>(lora_f32<float>(t.x[j].q[k]), hi, lo);
 #pragma unroll
                     for (int i = 0; i < MT; ++i)
                         lora_unit<sizeof(W) == 4>(acc[i][j], lora_f32<W>(t.w[2 * i].q[k]),
@@ -500,11 +531,18 @@ struct LoraShrink {
         __syncthreads();
     }
 
-    static __device__ __forceinline__ float sum(const Shared &s, int r, int tok) {
+    // The sum of rank r0 + r and token `token` at place tok, of the columns of units first .. u1.  What is not finite is
+    // made again in plain f32, since x in parts makes infinity less infinity of an infinity: 4096 tokens 138 us as
+    // without it, 0.5 ms if one has an infinite x; parts that infinity has (WIDE) for every x 138.7 us, 1000 tokens 32.8
+    // instead of 32.2.
+    static __device__ __forceinline__ float sum(const LoraArgs &p, const Shared &s, int a, int r0, int r, int tok,
+                                                int token, int first, int u1) {
         float v = 0.0f;
 #pragma unroll
         for (int k = 0; k < kKWarps; ++k) v += s.parts[k][r * kStride + tok];
-        return v;
+        if (fabsf(v) < INFINITY) return v;
+        const W *w = static_cast<const W *>(p.a) + (static_cast<int64_t>(a) * p.max_rank + r0 + r) * p.cols;
+        return lora_plain(w + 16 * first, p.x + token * p.x_stride + 16 * first, min(p.cols, 16 * u1) - 16 * first);
     }
 };
 
@@ -525,13 +563,13 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(LoraArgs p
         const int part = static_cast<int>(item % per_tile), split = part / chunks, r0 = part % chunks * kRanks;
         const int rank = tiles.rank;
         if (r0 >= rank) continue;
-        Shrink::run(p, shared, tiles.tokens, tiles.adapter, rank, r0, split * p.units,
-                    min((split + 1) * p.units, (p.cols + 15) / 16));
+        const int first = split * p.units, u1 = min(first + p.units, (p.cols + 15) / 16);
+        Shrink::run(p, shared, tiles.tokens, tiles.adapter, rank, r0, first, u1);
         for (int i = threadIdx.x; i < tiles.n * kRanks; i += kLoraThreads) {
-            const int tok = i / kRanks, r = i % kRanks;
+            const int r = i % kRanks, tok = i / kRanks, token = tiles.tokens[tok];
             if (r0 + r < rank)
-                p.h[(static_cast<int64_t>(split) * p.tokens + tiles.tokens[tok]) * lora_h_pitch(p.max_rank) + r0 + r] =
-                    Shrink::sum(shared, r, tok);
+                p.h[(static_cast<int64_t>(split) * p.tokens + token) * lora_h_pitch(p.max_rank) + r0 + r] =
+                    Shrink::sum(p, shared, tiles.adapter, r0, r, tok, token, first, u1);
         }
     }
 }
@@ -547,16 +585,17 @@ __host__ __device__ constexpr int lora_pitch(int rank) {
 // Element r of token tok's h, as hi + lo.
 template <int NT>
 __device__ __forceinline__ void lora_put(float *hs, int pitch, int tok, int r, float h) {
-    const uint32_t hi = lora_tf32(h);
+    uint32_t hi, lo;
+    lora_split<true>(h, hi, lo);
     hs[tok * pitch + r] = __uint_as_float(hi);
-    hs[(8 * NT + tok) * pitch + r] = __uint_as_float(lora_tf32(h - __uint_as_float(hi)));
+    hs[(8 * NT + tok) * pitch + r] = __uint_as_float(lo);
 }
 
 // Elements r .. r + 3 of token tok's h.
 template <int NT>
 __device__ __forceinline__ void lora_put(float *hs, int pitch, int tok, int r, const float4 &h) {
     uint32_t hi[4], lo[4];
-    lora_split(h, hi, lo);
+    lora_split<true>(h, hi, lo);
     *reinterpret_cast<uint4 *>(hs + tok * pitch + r) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
     *reinterpret_cast<uint4 *>(hs + (8 * NT + tok) * pitch + r) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
 }
@@ -832,12 +871,15 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_cluster_kernel(LoraArgs 
     if (rank == 0) return;  // the whole cluster
     float *mine = hs + 16 * lora_pitch<KU>(p.max_rank);
     const int units = (p.cols + 15) / 16, share = 2 * ((units + 2 * kLoraCluster - 1) / (2 * kLoraCluster));
+    const int first = min(part * share, units), u1 = min(first + share, units);
     for (int r0 = 0; r0 < rank; r0 += Shrink::kRanks) {
         if (r0) __syncthreads();  // the ranks before are read
-        Shrink::run(p, shared, tiles.tokens, tiles.adapter, rank, r0, part * share, min((part + 1) * share, units));
+        Shrink::run(p, shared, tiles.tokens, tiles.adapter, rank, r0, first, u1);
         for (int i = tid; i < n * Shrink::kRanks; i += kLoraThreads) {
             const int tok = i / Shrink::kRanks, r = i % Shrink::kRanks;
-            if (r0 + r < rank) mine[tok * p.max_rank + r0 + r] = Shrink::sum(shared, r, tok);
+            if (r0 + r < rank)
+                mine[tok * p.max_rank + r0 + r] =
+                    Shrink::sum(p, shared, tiles.adapter, r0, r, tok, tiles.tokens[tok], first, u1);
         }
     }
     cluster_arrive();

@@ -396,6 +396,9 @@ int32_t glmvx_dsa_attend(float *out, const int32_t *selected, const float *q_lat
  * max_rank, clamped) rows of A and columns of B are read, the rest may hold
  * anything.  Products and sums are f32 whatever the kind.  A token's result
  * does not depend on the other tokens' adapters and is the same every time.
+ * What is not finite in x[t] or h = A x[t] makes y[t] what the formula says
+ * (of F32 weights of B beyond 2048 an infinite h may make NaN instead); weights
+ * of B are finite.
  * tokens <= 2^20, rows and cols <= 2^22, adapters <= 2^24, max_rank <= 256.
  * y must not overlap x.  Pointers belong to the current device.  workspace:
  * device scratch of glmvx_lora_workspace_bytes(...) bytes (no less for more

@@ -326,3 +326,34 @@ def test_a_captured_call_of_many_tokens_replays(gpu_backend):
         g.close()
         for buf in list(bufs.values()) + [ws]:
             buf.close()
+
+
+@pytest.mark.parametrize('kind', [0, 1, 30])
+@pytest.mark.parametrize('tokens,adapters,cols', [(4, 2, 96), (40, 50, 96), (300, 3, 96), (5, 2, 31), (70, 2, 2100)])
+def test_infinities_are_the_formulas(gpu_backend, kind, tokens, adapters, cols):
+    """An infinite x makes what the formula makes of it: h and y infinite with its sign, NaN where signs or a zero meet
+    it.  Values next to the largest finite one stay finite and as exact as others."""
+    rank, rows = 3, 72
+    ids = np.arange(tokens) % adapters
+    ids[:4] = 0, 1, 0, 1
+    case = Case(tokens, rows, cols, adapters, rank, kind, ids=ids, ranks=[1 + 2 * (i % 2) for i in range(adapters)],
+                seed=cols)
+    a, b = case.a64.copy(), case.b64.copy()
+    a[0, 0, 7] = 1.5  # one TF32 part holds it
+    a[1, :, 5] = np.abs(a[1, :, 5])  # h of one sign
+    a[0, 0, 3] = 0.0
+    a[1, :, 11:13] *= 2.0 ** -7
+    b[1, :20] = np.abs(b[1, :20])  # ranks of one sign: infinite; mixed: NaN
+    case.a, case.a64 = pack(kind, a.astype(np.float32))
+    case.b, case.b64 = pack(kind, b.astype(np.float32))
+    big = np.finfo(np.float32).max
+    case.x[0, 7], case.x[1, 5], case.x[2, 3], case.x[3, 11:13] = np.inf, -np.inf, np.inf, (big, -big / 8)
+    with np.errstate(all='ignore'):
+        out = case.run(gpu_backend)[:, :rows].astype(np.float64)
+        want, tol = case.want()
+    assert np.isinf(want).any() and np.isnan(want).any()
+    assert np.array_equal(np.isnan(out), np.isnan(want))
+    assert np.array_equal(out[np.isinf(want)], want[np.isinf(want)])
+    fine = np.isfinite(want)
+    assert (np.abs(want[3][fine[3]]) > 1e30).any()
+    assert (np.abs(out[fine] - want[fine]) <= tol[fine]).all()
