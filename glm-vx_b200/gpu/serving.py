@@ -192,6 +192,7 @@ class BatchScheduler:
         req.finished = True
         if 0 <= req.slot < len(self.slots) and self.slots[req.slot] is req:
             self.slots[req.slot] = None
+            self._vacate(req)
         with self.lock:
             self.reserved -= req.reservation
             self.count -= 1
@@ -203,6 +204,17 @@ class BatchScheduler:
                                                'prefix_seconds': 0.0}})
         except queue.Full:
             pass
+
+    def _vacate(self, req):
+        """Takes the request's adapter and rules from its slot, which is stepped
+        with the others while it is idle."""
+        try:
+            if req.adapter is not None:
+                self.decoder.set_adapter(req.slot)
+            if req.rules:
+                self.decoder.rules.clear(req.slot)
+        except Exception as exc:  # the slot's next request does it again, or fails by it
+            self.error = str(exc)
 
     def _fail(self, exc, requests):
         """Ends the requests that the decoder's failure `exc` leaves without a result."""

@@ -502,3 +502,38 @@ def test_a_sequence_that_nothing_is_left_to_stays_at_its_end():
     dec.read_tokens = lambda: np.array(choices[steps.count('step') - 1], np.int32)
     out, _ = dec.generate([[1], [2], [3]], 4)
     assert out.tolist() == [[5, 5, -1, -1], [6, -1, -1, -1], [7, 8, 9, 2]]
+
+
+@pytest.mark.parametrize('how', ['length', 'exhausted', 'cancelled', 'error'])
+def test_a_finished_request_leaves_nothing_in_its_slot(serve, how):
+    """An idle slot is stepped with the others: it reads no adapter's weights, no mask and no history any more."""
+    sched = serve(2, 50, slots=2)
+    dec = sched.decoder
+    if how == 'error':
+        allowed = lambda output: 1 // 0 if output else None
+    else:
+        allowed = (lambda output: [] if output else [3]) if how == 'exhausted' else [3, 4]
+    req = sched.submit([4], 30, adapter=1, frequency_penalty=0.5, logit_bias={7: 2.0}, allowed=allowed)
+    if how == 'cancelled':
+        req.events.get(timeout=5)
+        sched.cancel(req)
+    assert collect(req, timeout=5)[1]['reason'] in (how, 'length')
+    assert dec.adapter == [None, None]
+    clean = HostRules(1, 50).rows[0]
+    assert [dict(row, history=[]) for row in dec.rules.rows] == [clean, clean]
+
+
+def test_a_slot_that_cannot_be_vacated_is_noted(serve):
+    sched = serve(1, 50, slots=1)
+    put = sched.decoder.set_adapter
+
+    def fails(b, slot=None):
+        if slot is None:
+            raise RuntimeError('as if')
+        put(b, slot)
+
+    sched.decoder.set_adapter = fails
+    tokens, done = collect(sched.submit([4], 3, adapter=0), timeout=5)
+    assert len(tokens) == 3 and done['reason'] == 'length' and sched.status()['error'] == 'as if'
+    sched.decoder.set_adapter = put
+    assert collect(sched.submit([4], 3), timeout=5)[0] == greedy(sched.decoder.table[0], 4, 3)
