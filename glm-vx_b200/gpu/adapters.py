@@ -15,6 +15,8 @@ the bank to its projections, gpu/serving.py `submit(adapter=slot)` picks one
 for a request.
 """
 
+import itertools
+
 import numpy as np
 
 from . import runtime as rt
@@ -75,7 +77,13 @@ class AdapterBank:
     30 (BF16), for calls of up to `max_tokens` rows.
 
     The calls of one bank share its workspace, so they belong on one stream
-    (the backend's by default)."""
+    (the backend's by default).
+
+    loaded[slot] is False while the slot is empty or about to change, else the
+    number of the load that filled it, another one each time: equal before
+    and after a step, it stood still meanwhile."""
+
+    _loads = itertools.count(1)
 
     def __init__(self, backend, shapes, slots, max_rank, kind=30, max_tokens=64):
         self.shapes = {str(k): (int(r), int(c)) for k, (r, c) in dict(shapes).items()}
@@ -156,15 +164,15 @@ class AdapterBank:
                 self._put(sb, b, slot * self.max_rank * rows * size)
             self._put(scales, np.array([scale], np.float32), 4 * slot)
             self._put(ranks, np.array([r], np.int32), 4 * slot)
-        self.loaded[slot] = True
+        self.loaded[slot] = next(self._loads)
 
     def unload(self, slot):
         """Empties `slot`: rows that still name it are left as the model has them."""
         slot = self._slot(slot)
         self.backend._begin()
+        self.loaded[slot] = False
         for _, _, ranks, _ in self._stacks.values():
             self._put(ranks, np.zeros(1, np.int32), 4 * slot)
-        self.loaded[slot] = False
 
     def add(self, name, y, x, ids, tokens, stream=None):
         """y[t] += the adapter ids[t]'s change of projection `name` at x[t], t <

@@ -65,6 +65,7 @@ class Request:
     slot: int = -1
     decode_seconds: float = 0.0
     adapter: int | None = None
+    adapter_load: int = 0
     rules: dict = field(default_factory=dict)
     allowed: object = None
     output: list = field(default_factory=list)
@@ -97,11 +98,12 @@ class BatchScheduler:
     # ---------------------------------------------------------- admission
     def submit(self, tokens, max_tokens, temperature=0.0, seed=0, *, adapter=None, repetition_penalty=1.0,
                presence_penalty=0.0, frequency_penalty=0.0, logit_bias=None, allowed=None):
-        """adapter: a loaded slot of the decoder's bank.  logit_bias: {token:
-        value to add, -inf to ban}.  allowed: the tokens that may be said, as a
-        boolean array over the vocabulary or token ids (copied here), or a
-        function from the list of tokens generated so far to such a mask (or
-        None: all)."""
+        """adapter: a loaded slot of the decoder's bank; should the adapter be
+        unloaded or replaced, the request ends with reason 'error'.
+        logit_bias: {token: value to add, -inf to ban}.  allowed: the tokens
+        that may be said, as a boolean array over the vocabulary or token ids
+        (copied here), or a function from the list of tokens generated so far
+        to such a mask (or None: all)."""
         cfg = self.config
         if not isinstance(tokens, list) or not tokens or any(type(t) is not int or not 0 <= t < cfg['vocab_size']
                                                              for t in tokens):
@@ -114,15 +116,18 @@ class BatchScheduler:
         if type(seed) is not int or seed < 0:
             raise ValueError('seed must be a nonnegative integer')
         rules, allowed = self._rules(repetition_penalty, presence_penalty, frequency_penalty, logit_bias, allowed)
+        load = 0
         if adapter is not None:
             bank = getattr(self.decoder, 'adapters', None)
-            if bank is None or type(adapter) is not int or not 0 <= adapter < bank.slots or not bank.loaded[adapter]:
+            if bank is not None and type(adapter) is int and 0 <= adapter < bank.slots:
+                load = bank.loaded[adapter]
+            if not load:
                 raise ValueError('adapter must be a loaded slot of the decoder\'s adapter bank')
         amount = len(tokens) + max_tokens
         if amount > min(cfg.get('max_position_embeddings', 2**31 - 1), self.decoder.capacity):
             raise ValueError('request exceeds context limit')
-        req = Request(tuple(tokens), max_tokens, float(temperature), seed, adapter=adapter, rules=rules,
-                      allowed=allowed)
+        req = Request(tuple(tokens), max_tokens, float(temperature), seed, adapter=adapter,
+                      adapter_load=load, rules=rules, allowed=allowed)
         req.reservation = amount
         req.rng = np.random.default_rng(seed)
         req.events = queue.Queue(maxsize=min(max_tokens + 2, self.max_pending_events))
@@ -205,6 +210,14 @@ class BatchScheduler:
         except queue.Full:
             pass
 
+    def _replaced(self, req):
+        """Whether the request's adapter is no longer the one it was submitted
+        with; then it has ended.  Seen after a step, no load or unload met it."""
+        if req.adapter is None or self.decoder.adapters.loaded[req.adapter] == req.adapter_load:
+            return False
+        self._finish(req, 'error', 'the adapter was unloaded or replaced')
+        return True
+
     def _vacate(self, req):
         """Takes the request's adapter and rules from its slot, which is stepped
         with the others while it is idle."""
@@ -249,6 +262,8 @@ class BatchScheduler:
                 self.slot_len[free] = 0
                 if getattr(self.decoder, 'adapters', None) is not None:
                     self.decoder.set_adapter(free, req.adapter)
+                if self._replaced(req):
+                    continue
                 if req.rules:
                     fixed = req.allowed if not callable(req.allowed) else None
                     self.decoder.rules.set(free, prompt=len(req.tokens), allowed=fixed, **req.rules)
@@ -303,6 +318,8 @@ class BatchScheduler:
                 self._fail(exc, active)
                 continue
             for r in active:
+                if self._replaced(r):
+                    continue
                 r.decode_seconds += dt
                 if r.cursor < len(r.tokens):
                     r.cursor += 1

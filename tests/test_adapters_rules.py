@@ -537,3 +537,61 @@ def test_a_slot_that_cannot_be_vacated_is_noted(serve):
     assert len(tokens) == 3 and done['reason'] == 'length' and sched.status()['error'] == 'as if'
     sched.decoder.set_adapter = put
     assert collect(sched.submit([4], 3), timeout=5)[0] == greedy(sched.decoder.table[0], 4, 3)
+
+
+def test_a_slot_is_empty_before_its_weights_change():
+    """Whoever compares a slot's load before and after a step sees every change that the step may have met."""
+    backend = QuietBackend()
+    bank = bank_without_device()
+    seen = []
+    buffer = lambda: SimpleNamespace(ptr=0, upload=lambda *args: seen.append(list(bank.loaded)))
+    bank.backend, bank._stacks = backend, {'a': tuple(buffer() for _ in range(4))}
+    weights = {'a': (np.zeros((1, 4)), np.zeros((6, 1)))}
+    bank.load(0, weights)
+    first = bank.loaded[0]
+    bank.load(1, weights)
+    assert first and bank.loaded[0] == first and bank.loaded[1] not in (False, first)
+    seen.clear()
+    bank.load(0, weights)
+    assert bank.loaded[0] not in (False, first, bank.loaded[1]) and seen and not any(s[0] for s in seen)
+    seen.clear()
+    bank.unload(1)
+    assert not bank.loaded[1] and seen and not any(s[1] for s in seen)
+
+
+def test_an_adapter_replaced_before_admission_ends_its_request_alone(serve):
+    """A request runs with the adapter that was there when it was submitted, not with what its slot holds later."""
+    sched = serve(2, 50, slots=1)
+    loaded = sched.decoder.adapters.loaded
+    loaded[0] = 11
+    with sched.lock:  # the worker admits after this block
+        req, fine = sched.submit([4], 3, adapter=0), sched.submit([4], 3)
+        loaded[0] = 12
+    tokens, done = collect(req, timeout=5)
+    assert tokens == [] and done['reason'] == 'error' and 'replaced' in done['error']
+    assert collect(fine, timeout=5)[0] == greedy(sched.decoder.table[0], 4, 3)
+    assert collect(sched.submit([4], 3, adapter=0), timeout=5)[0] == greedy(sched.decoder.table[1], 4, 3)
+
+
+@pytest.mark.parametrize('left', [False, 12])
+@pytest.mark.parametrize('prompt', [1, 9])
+def test_an_adapter_replaced_while_it_is_used_ends_its_request_alone(serve, left, prompt):
+    """No token comes from a step that a load or an unload may have met, be it in the prompt."""
+    sched = serve(2, 50, slots=1)
+    loaded, step, steps = sched.decoder.adapters.loaded, sched.decoder.step, []
+    loaded[0] = 11
+
+    def meets_a_load():
+        steps.append(len(steps))
+        if len(steps) == 5:
+            loaded[0] = left
+        step()
+
+    sched.decoder.step = meets_a_load
+    with sched.lock:
+        req, fine = sched.submit([4] * prompt, 20, adapter=0), sched.submit([4], 8)
+    tokens, done = collect(req, timeout=5)
+    assert done['reason'] == 'error' and 'replaced' in done['error']
+    assert tokens == greedy(sched.decoder.table[1], 4, 4 if prompt == 1 else 0)
+    assert collect(fine, timeout=5)[0] == greedy(sched.decoder.table[0], 4, 8)
+    assert sched.status()['error'] is None
