@@ -98,19 +98,20 @@ class AdapterBank:
         backend._begin()
         self._bufs = []
         self._stacks = {}
+        self.loaded = [False] * self.slots
         size = KINDS[self.kind][0]
         stream = backend.stream.handle
-        for name, (rows, cols) in self.shapes.items():
-            a = self._dev(self.slots * self.max_rank * cols * size)
-            b = self._dev(self.slots * self.max_rank * rows * size)
-            ranks, scales = self._dev(4 * self.slots), self._dev(4 * self.slots)
-            rt.call('glmvx_memset', ranks.ptr, 0, 4 * self.slots, stream)
-            rt.call('glmvx_memset', scales.ptr, 0, 4 * self.slots, stream)
-            self._stacks[name] = (a, b, ranks, scales)
-        need = int(self.lib.glmvx_lora_workspace_bytes(self.max_tokens, self.slots, self.max_rank))
-        self._workspace, self._workspace_bytes = self._dev(need), need
-        self.loaded = [False] * self.slots
-        backend.stream.synchronize()
+        with backend.device.lock:  # no other thread captures a step on the stream meanwhile
+            for name, (rows, cols) in self.shapes.items():
+                a = self._dev(self.slots * self.max_rank * cols * size)
+                b = self._dev(self.slots * self.max_rank * rows * size)
+                ranks, scales = self._dev(4 * self.slots), self._dev(4 * self.slots)
+                rt.call('glmvx_memset', ranks.ptr, 0, 4 * self.slots, stream)
+                rt.call('glmvx_memset', scales.ptr, 0, 4 * self.slots, stream)
+                self._stacks[name] = (a, b, ranks, scales)
+            need = int(self.lib.glmvx_lora_workspace_bytes(self.max_tokens, self.slots, self.max_rank))
+            self._workspace, self._workspace_bytes = self._dev(need), need
+            backend.stream.synchronize()
 
     def _dev(self, nbytes):
         buf = rt.DeviceBuffer(max(int(nbytes), 256))
@@ -188,8 +189,9 @@ class AdapterBank:
             self.backend.stream.handle if stream is None else stream), 'glmvx_lora_add')
 
     def close(self):
-        if self._bufs:
-            self.backend.stream.synchronize()
-        for buf in self._bufs:
-            buf.close()
-        self._bufs = []
+        with self.backend.device.lock:
+            if self._bufs:
+                self.backend.stream.synchronize()
+            for buf in self._bufs:
+                buf.close()
+            self._bufs = []

@@ -447,12 +447,13 @@ class ResidentDecoder:
         on the current hidden rows, for measuring it apart from the step."""
         L = self.layers[layer]
         g = rt.Graph(self.backend.stream)
-        g.begin()
-        try:
-            self._rmsnorm(self.n, self.x, L['in_norm'], self.hidden, self.eps)
-            self._attention(layer, L, None)
-        finally:
-            g.end()
+        with self.backend.device.lock:  # as in step_graph
+            g.begin()
+            try:
+                self._rmsnorm(self.n, self.x, L['in_norm'], self.hidden, self.eps)
+                self._attention(layer, L, None)
+            finally:
+                g.end()
         return g
 
     def _step_launches(self):

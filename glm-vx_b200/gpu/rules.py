@@ -69,10 +69,11 @@ class LogitRules:
         B, W = self.batch, (self.vocab + 31) // 32
         self.words = W
         self._masked = [None] * B  # whether sequence b has a mask (None: not yet said)
-        self._bufs = {name: rt.DeviceBuffer(nbytes) for name, nbytes in (
-            ('history', 4 * B * self.capacity), ('lens', 4 * B), ('prompts', 4 * B), ('penalties', 12 * B),
-            ('bias_ids', 4 * B * self.max_bias), ('bias_values', 4 * B * self.max_bias), ('bias_lens', 4 * B),
-            ('masks', 4 * B * W), ('mask_rows', 4 * B))}
+        sizes = (('history', 4 * B * self.capacity), ('lens', 4 * B), ('prompts', 4 * B), ('penalties', 12 * B),
+                 ('bias_ids', 4 * B * self.max_bias), ('bias_values', 4 * B * self.max_bias), ('bias_lens', 4 * B),
+                 ('masks', 4 * B * W), ('mask_rows', 4 * B))
+        with backend.device.lock:  # no other thread captures a step on the stream meanwhile
+            self._bufs = {name: rt.DeviceBuffer(nbytes) for name, nbytes in sizes}
         for b in range(B):
             self.clear(b)
 
@@ -171,8 +172,9 @@ class LogitRules:
             'glmvx_logits_select')
 
     def close(self):
-        if self._bufs:
-            self.backend.stream.synchronize()
-        for buf in self._bufs.values():
-            buf.close()
-        self._bufs = {}
+        with self.backend.device.lock:
+            if self._bufs:
+                self.backend.stream.synchronize()
+            for buf in self._bufs.values():
+                buf.close()
+            self._bufs = {}

@@ -595,3 +595,57 @@ def test_an_adapter_replaced_while_it_is_used_ends_its_request_alone(serve, left
     assert tokens == greedy(sched.decoder.table[1], 4, 4 if prompt == 1 else 0)
     assert collect(fine, timeout=5)[0] == greedy(sched.decoder.table[0], 4, 8)
     assert sched.status()['error'] is None
+
+
+class HeldLock:
+    """An RLock that knows how deep it is held."""
+
+    def __init__(self):
+        import threading
+        self.lock, self.depth = threading.RLock(), 0
+
+    def __enter__(self):
+        self.lock.acquire()
+        self.depth += 1
+
+    def __exit__(self, *exc):
+        self.depth -= 1
+        self.lock.release()
+
+
+def test_banks_and_rules_are_made_and_closed_outside_captures(monkeypatch):
+    """What they issue on the stream (and their memory's release) would join or end another thread's capture: all of
+    it holds the device's lock.  So does the capture of one layer's attention."""
+    from gpu import decoder
+    from gpu import runtime as rt
+    backend = QuietBackend()
+    backend.device.lock = HeldLock()
+    backend.lib = SimpleNamespace(glmvx_lora_workspace_bytes=lambda *args: 64)
+
+    class Buffer:
+        ptr = 0
+
+        def __init__(self, nbytes):
+            backend._note()
+
+        def upload(self, *args):
+            backend._note()
+
+        close = upload
+
+    monkeypatch.setattr(rt, 'DeviceBuffer', Buffer)
+    monkeypatch.setattr(rt, 'call', lambda name, *args: backend._note())
+    bank = AdapterBank(backend, {'a': (6, 4), 'b': (4, 4)}, 2, 3)
+    rules = LogitRules(backend, 2, 50, 8)
+    assert len(backend.held) >= 40 and all(backend.held)
+    backend.held.clear()
+    bank.close()
+    rules.close()
+    assert len(backend.held) >= 19 and all(backend.held)
+    backend.held.clear()
+    dec = decoder.ResidentDecoder.__new__(decoder.ResidentDecoder)
+    dec.backend, dec.layers, dec.n, dec.x, dec.hidden, dec.eps, dec._bufs = backend, [{'in_norm': 0}], 0, 0, 4, 0, []
+    dec._rmsnorm = dec._attention = backend._note
+    monkeypatch.setattr(rt, 'Graph', lambda stream: SimpleNamespace(begin=backend._note, end=backend._note))
+    dec.attention_graph()
+    assert backend.held == [True] * 4 and backend.device.lock.depth == 0

@@ -372,3 +372,39 @@ def test_a_bank_of_prompts_takes_every_number_of_tokens(gpu_backend, max_tokens)
         for buf in bufs:
             buf.close()
         bank.close()
+
+
+def test_a_bank_made_while_the_step_is_captured(gpu_backend, plain_logits):
+    """Another thread's new bank and rules wait for the capture's end, and so does their closing."""
+    import threading
+    import time
+    from gpu.adapters import AdapterBank, projection_shapes
+    from gpu.rules import LogitRules
+    made = []
+
+    def make():
+        made.append(AdapterBank(gpu_backend, projection_shapes(CONFIG), slots=2, max_rank=4))
+        made.append(LogitRules(gpu_backend, 2, 50, 8))
+
+    maker = threading.Thread(target=make)
+    closer = threading.Thread(target=lambda: [part.close() for part in made])
+    decs = [decoder(gpu_backend), decoder(gpu_backend)]
+    for dec, thread in zip(decs, (maker, closer)):
+        launches = dec._step_launches
+
+        def captured(thread=thread, launches=launches):
+            thread.start()
+            time.sleep(0.3)
+            assert thread.is_alive()
+            launches()
+
+        dec._step_launches = captured
+    try:
+        for dec, thread in zip(decs, (maker, closer)):
+            assert run(dec).tobytes() == plain_logits.tobytes()
+            thread.join(10)
+            assert not thread.is_alive() and len(made) == 2
+            assert run(dec).tobytes() == plain_logits.tobytes()
+    finally:
+        for dec in decs:
+            dec.close()
