@@ -16,6 +16,7 @@ for a request.
 """
 
 import itertools
+import threading
 
 import numpy as np
 
@@ -84,6 +85,11 @@ class AdapterBank:
     and after a step, it stood still meanwhile."""
 
     _loads = itertools.count(1)
+
+    def __new__(cls, *args, **kwargs):
+        bank = super().__new__(cls)
+        bank._changing = threading.RLock()  # one load or unload at a time: a slot is one adapter's as a whole
+        return bank
 
     def __init__(self, backend, shapes, slots, max_rank, kind=30, max_tokens=64):
         self.shapes = {str(k): (int(r), int(c)) for k, (r, c) in dict(shapes).items()}
@@ -155,25 +161,27 @@ class AdapterBank:
             wide = np.zeros((rows, self.max_rank), np.float32)
             wide[:, :r] = b
             ready[name] = (r, to_kind(a, self.kind), to_kind(wide, self.kind))
-        self.unload(slot)
-        for name, (r, a, b) in ready.items():
-            sa, sb, ranks, scales = self._stacks[name]
-            size = KINDS[self.kind][0]
-            rows, cols = self.shapes[name]
-            if r:
-                self._put(sa, a, slot * self.max_rank * cols * size)
-                self._put(sb, b, slot * self.max_rank * rows * size)
-            self._put(scales, np.array([scale], np.float32), 4 * slot)
-            self._put(ranks, np.array([r], np.int32), 4 * slot)
-        self.loaded[slot] = next(self._loads)
+        with self._changing:
+            self.unload(slot)
+            for name, (r, a, b) in ready.items():
+                sa, sb, ranks, scales = self._stacks[name]
+                size = KINDS[self.kind][0]
+                rows, cols = self.shapes[name]
+                if r:
+                    self._put(sa, a, slot * self.max_rank * cols * size)
+                    self._put(sb, b, slot * self.max_rank * rows * size)
+                self._put(scales, np.array([scale], np.float32), 4 * slot)
+                self._put(ranks, np.array([r], np.int32), 4 * slot)
+            self.loaded[slot] = next(self._loads)
 
     def unload(self, slot):
         """Empties `slot`: rows that still name it are left as the model has them."""
         slot = self._slot(slot)
-        self.backend._begin()
-        self.loaded[slot] = False
-        for _, _, ranks, _ in self._stacks.values():
-            self._put(ranks, np.zeros(1, np.int32), 4 * slot)
+        with self._changing:
+            self.backend._begin()
+            self.loaded[slot] = False
+            for _, _, ranks, _ in self._stacks.values():
+                self._put(ranks, np.zeros(1, np.int32), 4 * slot)
 
     def add(self, name, y, x, ids, tokens, stream=None):
         """y[t] += the adapter ids[t]'s change of projection `name` at x[t], t <

@@ -649,3 +649,27 @@ def test_banks_and_rules_are_made_and_closed_outside_captures(monkeypatch):
     monkeypatch.setattr(rt, 'Graph', lambda stream: SimpleNamespace(begin=backend._note, end=backend._note))
     dec.attention_graph()
     assert backend.held == [True] * 4 and backend.device.lock.depth == 0
+
+
+def test_two_loads_of_one_slot_do_not_mix():
+    """The slot holds one of the two adapters as a whole, and an unload between the two does not empty half of it."""
+    import threading
+    import time
+    bank, order = bank_without_device(), []
+    bank.backend, bank.shapes = QuietBackend(), {n: (6, 4) for n in 'abcd'}
+    bank._stacks = {n: 'ABrs' for n in bank.shapes}
+
+    def put(buf, array, offset):
+        order.append(threading.current_thread().name)
+        time.sleep(0.002)
+
+    bank._put = put
+    weights = {n: (np.ones((1, 4)), np.ones((6, 1))) for n in bank.shapes}
+    threads = [threading.Thread(target=bank.load, args=(0, weights), name=f'load {i}') for i in range(2)]
+    threads.append(threading.Thread(target=bank.unload, args=(0,), name='unload'))
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join(10)
+    assert len(order) == 2 * (4 + 16) + 4
+    assert sum(a != b for a, b in zip(order, order[1:])) == 2, order
