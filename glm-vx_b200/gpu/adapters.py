@@ -21,6 +21,7 @@ import threading
 import numpy as np
 
 from . import runtime as rt
+from .rules import to_f32
 
 MAX_RANK = 256
 # Storage of the stacks: GGML kind -> (bytes of a weight, name).
@@ -142,7 +143,7 @@ class AdapterBank:
         as the model has them.  Steps that run meanwhile see the slot empty,
         then with the projections that are already there."""
         slot = self._slot(slot)
-        scale = float(scale)
+        scale = to_f32(scale)
         if not np.isfinite(scale):
             raise ValueError('adapter scale must be finite')
         ready = {}
@@ -170,7 +171,7 @@ class AdapterBank:
                 if r:
                     self._put(sa, a, slot * self.max_rank * cols * size)
                     self._put(sb, b, slot * self.max_rank * rows * size)
-                self._put(scales, np.array([scale], np.float32), 4 * slot)
+                self._put(scales, np.array([scale]), 4 * slot)
                 self._put(ranks, np.array([r], np.int32), 4 * slot)
             self.loaded[slot] = next(self._loads)
 

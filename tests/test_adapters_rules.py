@@ -673,3 +673,10 @@ def test_two_loads_of_one_slot_do_not_mix():
         thread.join(10)
     assert len(order) == 2 * (4 + 16) + 4
     assert sum(a != b for a, b in zip(order, order[1:])) == 2, order
+
+
+@pytest.mark.parametrize('scale', [1e39, -1e39, pytest.param(10 ** 400, id='10^400'), float('nan'),
+                                   float('-inf')])
+def test_scales_beyond_float32_are_refused(scale):
+    with pytest.raises(ValueError, match='scale must be finite'):
+        bank_without_device().load(0, {}, scale)
