@@ -99,6 +99,8 @@ class AdapterBank:
             raise ValueError('an adapter bank needs projections with positive shapes')
         if self.slots < 1 or not 1 <= self.max_rank <= MAX_RANK or not 1 <= self.max_tokens <= 1 << 20:
             raise ValueError(f'slots and max_tokens must be positive, max_rank 1..{MAX_RANK}')
+        if self.slots > 1 << 24 or any(max(s) > 1 << 22 for s in self.shapes.values()):
+            raise ValueError('a bank has at most 2^24 slots, and projections of at most 2^22 rows and columns')
         if self.kind not in KINDS:
             raise ValueError('adapters are stored as kind 0 (F32), 1 (F16) or 30 (BF16)')
         self.backend, self.lib = backend, backend.lib

@@ -680,3 +680,12 @@ def test_two_loads_of_one_slot_do_not_mix():
 def test_scales_beyond_float32_are_refused(scale):
     with pytest.raises(ValueError, match='scale must be finite'):
         bank_without_device().load(0, {}, scale)
+
+
+@pytest.mark.parametrize('change', [dict(slots=(1 << 24) + 1), dict(shapes={'a': ((1 << 22) + 1, 4)}),
+                                    dict(shapes={'a': (4, (1 << 22) + 1)})])
+def test_banks_that_no_call_takes_are_refused(change):
+    args = dict(shapes={'a': (4, 4)}, slots=2, max_rank=4)
+    args.update(change)
+    with pytest.raises(ValueError, match='at most'):
+        AdapterBank(NoDevice(), **args)
