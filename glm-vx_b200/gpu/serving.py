@@ -325,8 +325,9 @@ class BatchScheduler:
                     r.cursor += 1
                     if r.cursor < len(r.tokens):
                         continue  # still inside the prompt: this step's output is not sampled
-                if r.rules and chosen[r.slot] < 0:
-                    self._finish(r, 'exhausted', 'no token is allowed')
+                if chosen[r.slot] < 0:  # no logit above -inf: by its rules, or the model's
+                    self._finish(r, *(('exhausted', 'no token is allowed') if r.rules else
+                                      ('error', 'nonfinite logits')))
                     continue
                 try:
                     token = self._sample(logits[r.slot], r) if r.temperature > 0 else int(chosen[r.slot])

@@ -689,3 +689,16 @@ def test_banks_that_no_call_takes_are_refused(change):
     args.update(change)
     with pytest.raises(ValueError, match='at most'):
         AdapterBank(NoDevice(), **args)
+
+
+def test_a_row_without_a_finite_logit_ends_its_request_alone(serve):
+    """A decoder with rules chooses -1 there for a request without rules too: no token, and nothing to feed."""
+    sched = serve(2, 50)
+    sched.decoder.table[0, 4, :] = -np.inf
+    sched.decoder.table[0, 7, 7] = 50.0
+    with sched.lock:
+        req, fine = sched.submit([4], 5), sched.submit([7], 5)
+    tokens, done = collect(req, timeout=5)
+    assert tokens == [] and done['reason'] == 'error'
+    assert collect(fine, timeout=5)[0] == [7] * 5
+    assert sched.status()['error'] is None
