@@ -2,7 +2,7 @@
 // rules.  Per token v of row b, in f32, each operation rounded once:
 //   seen in the history (or fed):  l = l > 0 ? l / repetition : l * repetition
 //   c times among the output:      l = l - c * frequency; if c: l = l - presence
-//   biased:                        l = l + bias   (of a token's entries the last holds)
+//   biased:                        l = l + bias   (of a token's entries the last holds; -inf bans, whatever l is)
 //   outside the grammar mask:      l = -inf
 // The choice is the lowest index of the largest l (a NaN counts as the
 // largest, its first index is taken, as numpy's argmax does), -1 if nothing
@@ -259,7 +259,10 @@ __global__ void __launch_bounds__(kSelThreads, 2) logits_select_kernel(SelArgs p
                 float x = in[slot_token[r]];
                 if (w & (kSelCount | kSelPrompt)) x = x > 0.0f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
                 if (n) x = __fsub_rn(__fsub_rn(x, __fmul_rn(static_cast<float>(n), freq)), pres);
-                if (entry) x = __fadd_rn(x, p.bias_values[static_cast<int64_t>(b) * p.bias_capacity + entry - 1]);
+                if (entry) {
+                    const float bias = p.bias_values[static_cast<int64_t>(b) * p.bias_capacity + entry - 1];
+                    x = bias == -INFINITY ? bias : __fadd_rn(x, bias);  // a ban, of an infinite logit too
+                }
                 slot[r] = __float_as_uint(x);
             }
             __syncthreads();

@@ -414,7 +414,7 @@ int32_t glmvx_lora_add(float *y, int64_t y_stride, const float *x, int64_t x_str
  * counterpart).  Row b's logits l[v], in f32 with one rounding per operation:
  *   v in the history, or fed:       l = l > 0 ? l / repetition : l * repetition
  *   v c > 0 times among the output: l = l - c * frequency - presence
- *   v biased:                       l = l + bias
+ *   v biased:                       l = l + bias; -inf if bias is, whatever l is
  *   mask bit of v clear:            l = -inf
  * go to out[b][v] (out may be logits), and the lowest index of the largest to
  * selected[b] (the first NaN when there is one, as numpy's argmax; -1 when

@@ -288,3 +288,26 @@ def test_vocabularies_around_the_blocks(gpu_backend, vocab):
 def test_many_rows(gpu_backend):
     """More rows than run at once, each with a CTA of its own."""
     Case(700, 1000, cap=12, penalties=True, bias=2, masks=4, seed=20).check(gpu_backend)
+
+
+@pytest.mark.parametrize('vocab', [64, 63])
+def test_a_ban_holds_whatever_the_logit_is(gpu_backend, vocab):
+    """-inf as a bias is the end of a token, also of one whose logit is infinite or no number, by itself or by its
+    penalties; with other biases those stay what the sum makes of them."""
+    case = Case(4, vocab, cap=4, lens=[2, 2, 0, 0], prompts=[0, 0, 0, 0], fed=[9, 9, -1, -1], penalties=True, bias=2,
+                bias_lens=[1, 1, 2, 2], seed=30)
+    case.history[:, :] = 9
+    case.penalties[:] = [1, 0, 0]
+    case.penalties[0] = [1e-38, 0, 0]  # 30 / 1e-38
+    case.penalties[1] = [1, 0, -3e38]  # three times
+    case.bias_ids[:] = [9, 5]
+    case.bias_values[:] = -np.inf
+    case.bias_values[2, 1] = 1.0
+    case.logits[:, 9], case.logits[2, 5] = 30.0, np.inf
+    case.logits[3, 9], case.logits[3, 5] = np.nan, np.inf
+    got = case.run(gpu_backend)
+    assert (got['out'][:, 9] == -np.inf).all() and got['out'][2, 5] == np.inf and got['out'][3, 5] == -np.inf
+    rest = np.delete(np.arange(vocab), [5, 9])
+    assert np.array_equal(got['out'][:, rest], case.logits[:, rest])
+    want = [int(np.argmax(np.where(np.arange(vocab) == 9, -np.inf, case.logits[b, :vocab]))) for b in (0, 1)]
+    assert got['selected'][:3].tolist() == want + [5] and got['selected'][3] == rest[np.argmax(case.logits[3, rest])]
