@@ -13,8 +13,13 @@
 // fragment that needs it: the order of K is free, so a lane takes eight
 // neighbouring columns where the fragment layout names t and t + 4 of each eight.
 // F16 and BF16 weights are TF32 numbers as they are; x, h and F32 weights go
-// in as two, hi + lo (x.hi, x.lo and, for F32, lo.hi products; 2^-22 of a term
-// is lost at most).  Sums are f32.
+// in as two, hi + lo, which leaves up to 2^-23 of them over.  With F32 weights the
+// product of the two lo, up to 2^-22, is not made: a product loses 2^-23 of
+// itself at most, of F32 weights 2^-21.  Sums are f32; the tensor cores cut what
+// an addition leaves over, so their chains end after 64 columns (of A) or ranks
+// (of B) and go on as rounded sums.  Error of the whole change against 64 bits,
+// in norms, at 6144 columns of rank 16: 3.4e-7 (F32 weights 4.9e-7), of rank 256
+// 5.8e-7 (7.9e-7); a plain f32 product's 1.5e-7 to 4.3e-7 and 3.1e-7 to 6.1e-7.
 //
 // Tokens of one adapter are gathered into tiles.  A token's sums are made in
 // the same order whatever tile and place it lands in.
@@ -48,6 +53,7 @@ constexpr int kLoraScan = 64;
 constexpr int kLoraMaxSplits = 32;
 constexpr int kLoraRankChunk = 64;   // ranks a shrink CTA takes
 constexpr int kLoraRows = 32;        // rows of B a warp takes at once
+constexpr int kLoraChain = 64;       // ranks that expand's sums go through in the tensor cores
 
 // A tile of the plan: n tokens of one adapter (the places behind them hold anything).
 constexpr int kLoraTile = 16;
@@ -607,14 +613,20 @@ __device__ __forceinline__ void lora_put(float *hs, int pitch, int tok, int r, c
 // time.  With VEC lanes whose rows are behind the last read the last ones and write nothing.
 // prepare() puts h into hs (lora_put, zero from the rank to the end of its chunk) and
 // synchronises; the first weights are on their way meanwhile.
-template <class W, int NT, int RG, int KU, bool VEC>
+template <class W, int NT, int RG, int KU, bool VEC, bool LONG>
 struct LoraExpand {
     static constexpr int kSpan = kLoraRows * RG, kChunk = 16 * KU;
+    // Chunks after which a chain of the tensor cores ends and goes on as a rounded f32 sum in shared memory, as in
+    // LoraShrink: in one chain the error of rank 256 against 64 bits is 1.4e-6 instead of 5.8e-7 (F32 weights 2.1e-6
+    // instead of 7.9e-7), 4096 tokens of rank 128 take 309 us instead of 324, 4 of rank 256 12.6 instead of 13.0.
+    // LONG is for stacks of more ranks than that: 1000 tokens of rank 64 take 32.3 us without it, 32.8 with it.
+    static constexpr int kSettle = kLoraChain / kChunk;
+    static constexpr int kSums = LONG ? 2 * RG * NT * kLoraThreads : 0;  // float4s of them
 
     template <class F>
-    static __device__ __forceinline__ void run(const LoraArgs &p, const float *hs, const int (&tokens)[8 * NT], int n,
-                                               int a, int rank, int row_first, int row_next, int steps,
-                                               const F &prepare) {
+    static __device__ __forceinline__ void run(const LoraArgs &p, const float *hs, float4 *sums,
+                                               const int (&tokens)[8 * NT], int n, int a, int rank, int row_first,
+                                               int row_next, int steps, const F &prepare) {
         const int t4 = 4 * (threadIdx.x & 3);
         const int chunks = (rank + kChunk - 1) / kChunk;
         const int lane_r = KU * t4;  // a lane has 4 KU neighbouring ranks of a chunk
@@ -741,7 +753,20 @@ struct LoraExpand {
                     }
                 }
             }
-            if (++chunk < chunks) return;
+            const bool last = ++chunk == chunks;
+            if (LONG && (last ? chunks > kSettle : chunk % kSettle == 0)) {
+#pragma unroll
+                for (int i = 0; i < 2 * RG * NT; ++i) {
+                    float4 &sum = sums[i * kLoraThreads + threadIdx.x];
+                    float *c = &acc[0][0][0][0] + 4 * i;
+                    const float4 v = chunk > kSettle ? sum : float4{};
+                    c[0] += v.x, c[1] += v.y, c[2] += v.z, c[3] += v.w;
+                    if (last) continue;
+                    sum = make_float4(c[0], c[1], c[2], c[3]);
+                    c[0] = c[1] = c[2] = c[3] = 0.0f;
+                }
+            }
+            if (!last) return;
             chunk = 0;
 #pragma unroll
             for (int q = 0; q < RG; ++q) {
@@ -775,10 +800,10 @@ struct LoraExpand {
 };
 
 // The tiles' steps in one row, a run of them a CTA; h from the workspace, its parts joined in order.
-template <class W, int NT, int RG, int KU, bool VEC>
+template <class W, int NT, int RG, int KU, bool VEC, bool LONG>
 __global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(LoraArgs p) {
-    using Expand = LoraExpand<W, NT, RG, KU, VEC>;
-    extern __shared__ __align__(16) float hs[];  // [2][8 NT][pitch]: hi, lo
+    using Expand = LoraExpand<W, NT, RG, KU, VEC, LONG>;
+    extern __shared__ __align__(16) float hs[];  // [2][8 NT][pitch]: hi, lo; the sums of ranks above 64
     __shared__ LoraTiles<8 * NT> tiles;
     constexpr int kNext = kLoraWarps * Expand::kSpan;
     const int tid = threadIdx.x, warp = tid >> 5;
@@ -795,7 +820,8 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(LoraArgs p
         const int rank = tiles.rank;
         if (rank == 0) continue;
         const int row_first = (first * kLoraWarps + warp) * Expand::kSpan;
-        Expand::run(p, hs, tiles.tokens, tiles.n, tiles.adapter, rank, row_first, kNext, steps, [&]() {
+        float4 *sums = reinterpret_cast<float4 *>(hs + 16 * NT * lora_pitch<KU>(p.max_rank));
+        Expand::run(p, hs, sums, tiles.tokens, tiles.n, tiles.adapter, rank, row_first, kNext, steps, [&]() {
             if (!waited) grid_dependency_wait();  // h comes from the kernel before
             waited = true;
             // Each quad of ranks is summed by 2^team lanes, four parts in flight in each: the joining is bound by
@@ -856,11 +882,11 @@ __device__ __forceinline__ float cluster_load(const float *at, uint32_t rank) { 
     return v;
 }
 
-template <class W, int MT, int MW, int RG, int KU, bool VEC>
+template <class W, int MT, int MW, int RG, int KU, bool VEC, bool LONG>
 __global__ void __launch_bounds__(kLoraThreads, 2) lora_cluster_kernel(LoraArgs p) {
     using Shrink = LoraShrink<W, MT, MW, 1, VEC>;
-    using Expand = LoraExpand<W, 1, RG, KU, VEC>;
-    extern __shared__ __align__(16) float hs[];  // [2][8][pitch]: hi, lo; then this CTA's sums [8][max_rank]
+    using Expand = LoraExpand<W, 1, RG, KU, VEC, LONG>;
+    extern __shared__ __align__(16) float hs[];  // [2][8][pitch]: hi, lo; this CTA's h [8][max_rank]; sums of ranks above 64
     __shared__ LoraTiles<8> tiles;
     __shared__ typename Shrink::Shared shared;
     const int tid = threadIdx.x, part = blockIdx.x % kLoraCluster, tile = blockIdx.x / kLoraCluster;
@@ -886,7 +912,8 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_cluster_kernel(LoraArgs 
     const int row_first = (part * kLoraWarps + (tid >> 5)) * Expand::kSpan;
     const int row_next = kLoraCluster * kLoraWarps * Expand::kSpan;
     const int steps = row_first < p.rows ? (p.rows - row_first + row_next - 1) / row_next : 0;
-    Expand::run(p, hs, tiles.tokens, n, tiles.adapter, rank, row_first, row_next, steps, [&]() {
+    float4 *sums = reinterpret_cast<float4 *>(mine + 8 * p.max_rank);
+    Expand::run(p, hs, sums, tiles.tokens, n, tiles.adapter, rank, row_first, row_next, steps, [&]() {
         cluster_wait();
         const int width = (rank + Expand::kChunk - 1) / Expand::kChunk * Expand::kChunk;
         for (int i = tid; i < 8 * width; i += kLoraThreads) {
@@ -968,20 +995,25 @@ int32_t lora_shrink(const LoraArgs &p, dim3 grid, bool vec, cudaStream_t stream)
     return lora_start(kernel, grid, 0, p, p.tiles, stream, "lora_shrink_kernel");
 }
 
-template <class W, int NT, int RG, int KU>
+template <class W, int NT, int RG, int KU, bool LONG>
 int32_t lora_expand(const LoraArgs &p, dim3 grid, bool vec, cudaStream_t stream) {
-    const size_t smem = sizeof(float) * 2 * 8 * NT * lora_pitch<KU>(p.max_rank);
-    const auto kernel = vec ? lora_expand_kernel<W, NT, RG, KU, true> : lora_expand_kernel<W, NT, RG, KU, false>;
-    if (const int32_t rc = allow_dynamic_smem(kernel, smem, "lora_expand smem")) return rc;
+    constexpr int sums = LoraExpand<W, NT, RG, KU, true, LONG>::kSums;
+    const size_t smem = sizeof(float) * 2 * 8 * NT * lora_pitch<KU>(p.max_rank) + sizeof(float4) * sums;
+    const auto kernel =
+        vec ? lora_expand_kernel<W, NT, RG, KU, true, LONG> : lora_expand_kernel<W, NT, RG, KU, false, LONG>;
+    if (const int32_t rc = allow_dynamic_smem(kernel, smem, "lora_expand smem", sizeof(LoraTiles<8 * NT>))) return rc;
     return lora_start(kernel, grid, smem, p, true, stream, "lora_expand_kernel");
 }
 
-template <class W, int MT, int MW, int RG, int KU>
+template <class W, int MT, int MW, int RG, int KU, bool LONG>
 int32_t lora_cluster(const LoraArgs &p, int tiles, bool vec, cudaStream_t stream) {
     const auto kernel =
-        vec ? lora_cluster_kernel<W, MT, MW, RG, KU, true> : lora_cluster_kernel<W, MT, MW, RG, KU, false>;
-    const size_t smem = sizeof(float) * (16 * lora_pitch<KU>(p.max_rank) + 8 * p.max_rank);
-    if (const int32_t rc = allow_dynamic_smem(kernel, smem, "lora_cluster smem")) return rc;
+        vec ? lora_cluster_kernel<W, MT, MW, RG, KU, true, LONG> : lora_cluster_kernel<W, MT, MW, RG, KU, false, LONG>;
+    constexpr int sums = LoraExpand<W, 1, RG, KU, true, LONG>::kSums;
+    const size_t smem =
+        sizeof(float) * (16 * lora_pitch<KU>(p.max_rank) + 8 * p.max_rank) + sizeof(float4) * sums;
+    constexpr size_t fixed = sizeof(LoraTiles<8>) + sizeof(typename LoraShrink<W, MT, MW, 1, true>::Shared);
+    if (const int32_t rc = allow_dynamic_smem(kernel, smem, "lora_cluster smem", fixed)) return rc;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = kLoraCluster;
@@ -1005,9 +1037,10 @@ int32_t lora_launch(LoraArgs &p, bool vec_a, bool vec_b, cudaStream_t stream) {
     if (NT == 1 && tiles * kLoraCluster <= sms && weights <= kLoraSmall) {
         const bool vec = vec_a && vec_b;
         constexpr int kTwo = sizeof(W) == 4 ? 1 : 2;
-        if (p.max_rank <= 16) return lora_cluster<W, 1, 1, kTwo, 1>(p, tiles, vec, stream);
-        if (p.max_rank <= 32) return lora_cluster<W, 2, 1, 1, kTwo>(p, tiles, vec, stream);
-        return lora_cluster<W, 2, 2, 1, kTwo>(p, tiles, vec, stream);
+        if (p.max_rank <= 16) return lora_cluster<W, 1, 1, kTwo, 1, false>(p, tiles, vec, stream);
+        if (p.max_rank <= 32) return lora_cluster<W, 2, 1, 1, kTwo, false>(p, tiles, vec, stream);
+        if (p.max_rank <= kLoraChain) return lora_cluster<W, 2, 2, 1, kTwo, false>(p, tiles, vec, stream);
+        return lora_cluster<W, 2, 2, 1, kTwo, true>(p, tiles, vec, stream);
     }
     if (p.tiles) {
         static_assert(NT == 1 || 8 * NT == kLoraTile);
@@ -1041,9 +1074,11 @@ int32_t lora_launch(LoraArgs &p, bool vec_a, bool vec_b, cudaStream_t stream) {
     // of rank 64 187, by 16 at a time 146 and 206; F32 weights fill 16 bytes with 16 ranks.  Rank 16 and few tokens
     // take twice the rows a step: 64 tokens 20.8 us against 23.7.
     const dim3 out = ctas(lora_ceil(p.rows, kLoraWarps * kLoraRows));
+    constexpr int kWide = sizeof(W) == 4 ? 1 : 2;
+    if (p.max_rank > kLoraChain) return lora_expand<W, NT, 1, kWide, true>(p, out, vec_b, stream);
     if (sizeof(W) == 4 || p.max_rank <= 16)
-        return lora_expand<W, NT, NT == 1 && sizeof(W) == 2 ? 2 : 1, 1>(p, out, vec_b, stream);
-    return lora_expand<W, NT, 1, sizeof(W) == 4 ? 1 : 2>(p, out, vec_b, stream);
+        return lora_expand<W, NT, NT == 1 && sizeof(W) == 2 ? 2 : 1, 1, false>(p, out, vec_b, stream);
+    return lora_expand<W, NT, 1, kWide, false>(p, out, vec_b, stream);
 }
 
 }  // namespace

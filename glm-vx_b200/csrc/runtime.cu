@@ -62,8 +62,8 @@ int sm_count() {
     return cached[dev];
 }
 
-int32_t allow_dynamic_smem(const void *kernel, size_t bytes, const char *name) {
-    if (bytes <= 48 * 1024) return kOk;  // below the default limit nothing needs raising
+int32_t allow_dynamic_smem(const void *kernel, size_t bytes, const char *name, size_t fixed) {
+    if (bytes + fixed <= 48 * 1024) return kOk;  // below the default limit nothing needs raising
     int dev = 0;
     GLMVX_CUDA(cudaGetDevice(&dev));
     static std::mutex mu;

@@ -394,8 +394,11 @@ int32_t glmvx_dsa_attend(float *out, const int32_t *selected, const float *q_lat
  * a: [adapters][max_rank][cols], b: [adapters][rows][max_rank], both of one
  * GGML kind: 0 F32, 1 F16, 30 BF16; of adapter a the first ranks[a] (0 ..
  * max_rank, clamped) rows of A and columns of B are read, the rest may hold
- * anything.  Products and sums are f32 whatever the kind.  A token's result
- * does not depend on the other tokens' adapters and is the same every time.
+ * anything.  Sums are f32 whatever the kind; a product loses up to 2^-23 of
+ * itself before it is added (F32 weights: 2^-21) and up to 64 at a time are
+ * added with what is left over cut, not rounded: of normal data the whole
+ * change is off by less than 1e-6 of its norm.  A token's result does not depend on the other
+ * tokens' adapters and is the same every time.
  * What is not finite in x[t] or h = A x[t] makes y[t] what the formula says
  * (of F32 weights of B beyond 2048 an infinite h may make NaN instead); weights
  * of B are finite.

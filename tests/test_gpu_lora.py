@@ -357,3 +357,37 @@ def test_infinities_are_the_formulas(gpu_backend, kind, tokens, adapters, cols):
     fine = np.isfinite(want)
     assert (np.abs(want[3][fine[3]]) > 1e30).any()
     assert (np.abs(out[fine] - want[fine]) <= tol[fine]).all()
+
+
+@pytest.mark.parametrize('kind', [0, 1, 30])
+@pytest.mark.parametrize('tokens', [4, 40, 300])
+@pytest.mark.parametrize('rank', [16, 256])
+def test_long_sums_do_not_drift(gpu_backend, kind, tokens, rank):
+    """The norm of the whole change's error, which a bound for every element is too wide to see.
+
+    A tensor core cuts what an addition leaves over: half of 2^-23 of the sum at the mean, toward zero.  Through 64
+    normal products, eight at a time, the sum grows as the root of their number; 0.8 sqrt(8 i) for i = 1 .. 8, added
+    up, is 36 of a product's size where the sum itself has 8: 4.5 * 2^-24 of it, for each of the m products of parts
+    that a step adds one after another (2; 3 with F32 weights).  Chains end there and go on as rounded sums, whose
+    errors are of one sign with what they cut: A's 6144 columns lose that share of h, B's ranks that of y (a quarter of
+    the ranks an eighth: 16 are cut to 1.1 * 2^-24).  The parts leave 2^-23 of x and of h over."""
+    rows, cols, adapters = 256, 6144, 3
+    ids = np.arange(tokens) % adapters
+    case = Case(tokens, rows, cols, adapters, rank, kind, ids=ids, ranks=[rank] * adapters, seed=rank)
+    case.y[:] = 0
+    want, _ = case.want()
+    off = np.linalg.norm(case.run(gpu_backend) - want) / np.linalg.norm(want)
+    m = 3 if kind == 0 else 2
+    assert off <= m * (4.5 + (4.5 if rank >= 64 else 1.1)) * 2.0 ** -24 + 2.0 ** -22, off
+
+
+@pytest.mark.parametrize('kind', [0, 1, 30])
+@pytest.mark.parametrize('max_rank', [64, 65, 72, 128, 136, 255])
+def test_ranks_around_the_chains(gpu_backend, kind, max_rank):
+    """Stacks of up to 64 ranks and of more, whose adapters end before, at and after a multiple of 64."""
+    ranks = [min(r, max_rank) for r in (1, 63, 64, 65, 127, 128, 129, 192, 255)]
+    for tokens, cols, rows in ((9, 96, 132), (70, 100, 67)):
+        Case(tokens, rows, cols, 9, max_rank, kind, ids=np.arange(tokens) % 9, ranks=ranks,
+             seed=max_rank).check(gpu_backend)
+    case = Case(3, 64, 64, 3, max_rank, kind, ids=[2, 0, 2], ranks=ranks[-3:], seed=max_rank)
+    assert case.check(gpu_backend).tobytes() == case.run(gpu_backend).tobytes()
