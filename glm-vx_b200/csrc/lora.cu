@@ -537,10 +537,10 @@ struct LoraShrink {
         __syncthreads();
     }
 
-    // The sum of rank r0 + r and token `token` at place tok, of the columns of units first .. u1.  What is not finite is
-    // made again in plain f32, since x in parts makes infinity less infinity of an infinity: 4096 tokens 138 us as
-    // without it, 0.5 ms if one has an infinite x; parts that infinity has (WIDE) for every x 138.7 us, 1000 tokens 32.8
-    // instead of 32.2.
+    // The sum of rank r0 + r and token `token` at place tok, of the columns of units first .. u1.  What is not finite
+    // is made again in plain f32, since x in parts makes infinity less infinity of an infinity: 4096 tokens 138 us as
+    // without it, 0.5 ms if one has an infinite x; parts that infinity has (WIDE) for every x 138.7 us, 1000 tokens
+    // 32.8 instead of 32.2.
     static __device__ __forceinline__ float sum(const LoraArgs &p, const Shared &s, int a, int r0, int r, int tok,
                                                 int token, int first, int u1) {
         float v = 0.0f;
@@ -803,7 +803,7 @@ struct LoraExpand {
 template <class W, int NT, int RG, int KU, bool VEC, bool LONG>
 __global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(LoraArgs p) {
     using Expand = LoraExpand<W, NT, RG, KU, VEC, LONG>;
-    extern __shared__ __align__(16) float hs[];  // [2][8 NT][pitch]: hi, lo; the sums of ranks above 64
+    extern __shared__ __align__(16) float hs[];  // [2][8 NT][pitch]: hi, lo; LONG: sums
     __shared__ LoraTiles<8 * NT> tiles;
     constexpr int kNext = kLoraWarps * Expand::kSpan;
     const int tid = threadIdx.x, warp = tid >> 5;
@@ -886,7 +886,7 @@ template <class W, int MT, int MW, int RG, int KU, bool VEC, bool LONG>
 __global__ void __launch_bounds__(kLoraThreads, 2) lora_cluster_kernel(LoraArgs p) {
     using Shrink = LoraShrink<W, MT, MW, 1, VEC>;
     using Expand = LoraExpand<W, 1, RG, KU, VEC, LONG>;
-    extern __shared__ __align__(16) float hs[];  // [2][8][pitch]: hi, lo; this CTA's h [8][max_rank]; sums of ranks above 64
+    extern __shared__ __align__(16) float hs[];  // [2][8][pitch]: hi, lo; the CTA's h [8][max_rank]; LONG: sums
     __shared__ LoraTiles<8> tiles;
     __shared__ typename Shrink::Shared shared;
     const int tid = threadIdx.x, part = blockIdx.x % kLoraCluster, tile = blockIdx.x / kLoraCluster;

@@ -408,3 +408,52 @@ def test_a_bank_made_while_the_step_is_captured(gpu_backend, plain_logits):
     finally:
         for dec in decs:
             dec.close()
+
+
+def test_a_served_adapter_that_is_replaced(gpu_backend):
+    """Its request ends with an error, its neighbours say what they say alone, and the slot is left as a plain one."""
+    import threading
+    from gpu.adapters import AdapterBank, projection_shapes
+    from gpu.rules import LogitRules
+    from gpu.serving import BatchScheduler, collect
+    bank = AdapterBank(gpu_backend, projection_shapes(CONFIG), slots=2, max_rank=8, max_tokens=len(PROMPTS))
+    bank.load(0, adapter(5, all_names(), 8), SCALE)
+    rules = LogitRules(gpu_backend, len(PROMPTS), CONFIG['vocab_size'], capacity=40)
+    dec = decoder(gpu_backend, adapters=bank, rules=rules)
+    sched = BatchScheduler(dec)
+    said, loaded = threading.Event(), threading.Event()
+
+    def pause(output):  # the worker waits here for the load, between two steps
+        if len(output) == 3:
+            said.set()
+            loaded.wait(10)
+        return None
+
+    try:
+        alone = collect(sched.submit(list(PROMPTS[0]), 12))[0]
+        mine = collect(sched.submit(list(PROMPTS[1]), 12, adapter=0))[0]
+        with sched.lock:
+            fine, ends = sched.submit(list(PROMPTS[0]), 12), sched.submit(list(PROMPTS[1]), 12, adapter=0,
+                                                                          allowed=pause)
+        assert said.wait(10)
+        bank.load(0, adapter(6, all_names(), 8), SCALE)
+        loaded.set()
+        tokens, done = collect(ends)
+        assert done['reason'] == 'error' and 'replaced' in done['error'] and tokens == mine[:3]
+        assert collect(fine)[0] == alone
+        ids = np.zeros(len(PROMPTS), np.int32)
+        dec.adapter_ids.download(ids, gpu_backend.stream.handle)
+        gpu_backend.stream.synchronize()
+        assert (ids == -1).all()
+        assert collect(sched.submit(list(PROMPTS[1]), 12, adapter=0))[0] != mine
+        bank.unload(0)
+        with pytest.raises(ValueError, match='adapter'):
+            sched.submit(list(PROMPTS[1]), 12, adapter=0)
+        assert collect(sched.submit(list(PROMPTS[0]), 12))[0] == alone and sched.status()['error'] is None
+    finally:
+        loaded.set()
+        sched.close()
+        dec.check()
+        dec.close()
+        rules.close()
+        bank.close()

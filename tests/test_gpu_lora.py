@@ -391,3 +391,38 @@ def test_ranks_around_the_chains(gpu_backend, kind, max_rank):
              seed=max_rank).check(gpu_backend)
     case = Case(3, 64, 64, 3, max_rank, kind, ids=[2, 0, 2], ranks=ranks[-3:], seed=max_rank)
     assert case.check(gpu_backend).tobytes() == case.run(gpu_backend).tobytes()
+
+
+@pytest.mark.parametrize('tokens,adapters,used', [(1 << 20, 1, 1), (1 << 20, 3, 2), (3000, 1 << 20, 1 << 20),
+                                                  (40, 1 << 24, 1 << 24)])
+def test_the_largest_numbers_of_tokens_and_adapters(gpu_backend, tokens, adapters, used):
+    """Against 64 bits: sums of 8 and 1 products, off by (8 / 8 + 40) * 2^-23 + 3 * 2^-22 of their terms each."""
+    rows, cols, s = 4, 8, gpu_backend.stream
+    rng = np.random.default_rng(tokens)
+    ids = rng.integers(adapters - used, adapters, tokens).astype(np.int32)
+    ids[::7] = -1
+    x = rng.normal(size=(tokens, cols)).astype(np.float32)
+    a, b = (rng.normal(size=(adapters, n)).astype(np.float16) for n in (cols, rows))
+    need = gpu_backend.lib.glmvx_lora_workspace_bytes(tokens, adapters, 1)
+    host = dict(y=np.zeros((tokens, rows), np.float32), x=x, ids=ids, a=a, b=b, ranks=np.ones(adapters, np.int32),
+                scales=np.full(adapters, 2.0, np.float32), ws=np.full(need, 0xff, np.uint8))
+    dev = {n: rt.DeviceBuffer(v.nbytes) for n, v in host.items()}
+    try:
+        for n, v in host.items():
+            dev[n].upload(v, s.handle)
+        rt.call('glmvx_lora_add', dev['y'].ptr, rows, dev['x'].ptr, cols, dev['ids'].ptr, 1, dev['a'].ptr,
+                dev['b'].ptr, dev['ranks'].ptr, dev['scales'].ptr, tokens, rows, cols, adapters, 1, dev['ws'].ptr,
+                need, s.handle)
+        out = np.empty_like(host['y'])
+        dev['y'].download(out, s.handle)
+        s.synchronize()
+    finally:
+        for buf in dev.values():
+            buf.close()
+    at, has = np.maximum(ids, 0), (ids >= 0)[:, None]
+    h = np.einsum('tc,tc->t', x.astype(np.float64), a[at].astype(np.float64))[:, None]
+    mass = np.einsum('tc,tc->t', np.abs(x).astype(np.float64), np.abs(a[at]).astype(np.float64))[:, None]
+    want = np.where(has, 2 * h * b[at].astype(np.float64), 0.0)
+    off = 41 * 2.0 ** -23 + 3 * 2.0 ** -22
+    tol = np.where(has, 2 * (2 * off + off * off) * mass * np.abs(b[at]).astype(np.float64), 0.0)
+    assert (np.abs(out - want) <= tol).all()
