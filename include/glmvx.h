@@ -419,9 +419,10 @@ int32_t glmvx_lora_add(float *y, int64_t y_stride, const float *x, int64_t x_str
  *   v c > 0 times among the output: l = l - c * frequency - presence
  *   v biased:                       l = l + bias; -inf if bias is, whatever l is
  *   mask bit of v clear:            l = -inf
- * go to out[b][v] (out may be logits), and the lowest index of the largest to
- * selected[b] (the first NaN when there is one, as numpy's argmax; -1 when
- * nothing is above -inf).  Strides in elements.  Each group may be NULL:
+ * go to out[b][v] (out may be logits, else they do not overlap), and the
+ * lowest index of the largest to selected[b] (the first NaN when there is one,
+ * as numpy's argmax; -1 when nothing is above -inf).  Strides in elements.
+ * Each group may be NULL:
  *   history   history[b][history_capacity] token ids, the first
  *             history_lens[b] valid, of those the first prompt_lens[b] (NULL:
  *             none) the prompt, the rest output; ids outside the vocabulary
