@@ -48,9 +48,10 @@ int *device_error_word();
 int sm_count();
 
 // Allows `kernel` (a __global__ function) `bytes` of dynamic shared memory
-// beside the `fixed` that it declares, on the CURRENT device.  The attribute belongs to the function in one device's
-// context, so it is raised once per (device, kernel) and size, under a lock
-// (several host threads and several devices may launch the same kernel).
+// beside the `fixed` that it declares, on the CURRENT device.  The attribute
+// belongs to the function in one device's context, so it is raised once per
+// (device, kernel) and size, under a lock (several host threads and several
+// devices may launch the same kernel).
 int32_t allow_dynamic_smem(const void *kernel, size_t bytes, const char *name, size_t fixed = 0);
 template <class K>
 inline int32_t allow_dynamic_smem(K *kernel, size_t bytes, const char *name, size_t fixed = 0) {
